@@ -273,6 +273,55 @@ B200_API int b200_attention_bwd_noalloc(b200_stream_t stream, const void* q, con
                                         const int64_t stride_dv[4], float sm_scale, int causal, int dtype);
 B200_API long long b200_attention_bwd_noalloc_capacity(void);
 
+/* ---- Serving: packed prompts, a paged 8-bit cache, single tokens over it.  (No counterpart in the
+ * reference, whose attention takes dense batches of one length and one head count.) */
+
+/* Attention of whole prompts packed behind one another, with grouped heads: q, o [T, Hq, D] and k, v
+ * [T, Hkv, D] of `dtype` (F16 or BF16), Hq a multiple of Hkv, query head h reads k/v head h / (Hq / Hkv);
+ * sequence b is the rows cu_seqlens[b] .. cu_seqlens[b + 1] (a DEVICE array of batch + 1 ints that do not
+ * decrease; what lies outside [0, T] is cut off).  Each sequence attends to itself, up to the row itself
+ * when `causal`.  Strides are {token, head, d} in elements, the d stride 1, the others multiples of 8; base
+ * addresses 16-byte aligned; D is 64, 128 or 256.  m (may be NULL): [Hq, T] fp32, the base-2 log-sum-exp of
+ * b200_attention_fwd.  Rows of o and m that belong to no sequence are left as they were (zero_rest = 0) or
+ * set to zero and -inf (zero_rest = 1).  Values of one sequence never reach another, infinities and NaN
+ * included.  A launch draws a work counter like b200_attention_fwd's. */
+B200_API int b200_attention_varlen_fwd(b200_stream_t stream, const void* q, const void* k, const void* v, void* o,
+                                       float* m, const int* cu_seqlens, int batch, int T, int Hq, int Hkv, int D,
+                                       const int64_t stride_q[3], const int64_t stride_k[3], const int64_t stride_v[3],
+                                       const int64_t stride_o[3], float sm_scale, int causal, int dtype, int zero_rest);
+
+/* The cache: k_cache and v_cache [pages][Hkv][page_size][D] of e4m3 values, contiguous, 16-byte aligned;
+ * k_scale and v_scale [pages][Hkv] fp32, powers of two; a value is byte * scale of its page and head.
+ * page_size is 16, 32, 64 or 128 tokens; D is 64, 128 or 256.  Token t of sequence b is row t % page_size of page
+ * page_table[b * table_stride + t / page_size] (a DEVICE array of ints, max_pages of them per sequence).  An
+ * entry outside [0, pages) names no page: what would be written there is dropped, what would be read there is
+ * left out of the softmax.
+ *
+ * b200_kv_append writes new rows k, v [T, Hkv, D] (F16 or BF16, strides {token, head, d} as above).  With
+ * cu_seqlens (DEVICE, batch + 1 ints) sequence b's new rows are cu_seqlens[b] .. cu_seqlens[b + 1]; with NULL
+ * every sequence has one (T == batch).  seq_lens[b] (DEVICE) is the sequence's length WITH the new rows,
+ * which become its last tokens.  The scale of a page and head is 2^e, e the smallest integer >= -126 with
+ * |x| <= 448 * 2^e for every finite x of the rows written to it, raised (and the rows held already rounded
+ * anew) when later rows need more; a row is stored as e4m3(x / scale), round to nearest even; values that are
+ * not finite are stored as NaN.  A page that gets its row 0 starts a new scale.  Pages that two sequences
+ * of one call write to are the caller's mistake (the result is one of the two, or a mixture). */
+B200_API int b200_kv_append(b200_stream_t stream, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                            int pages, int page_size, const int* page_table, int64_t table_stride, int max_pages,
+                            const int* seq_lens, const void* k, const void* v, const int* cu_seqlens, int batch, int T,
+                            int Hkv, int D, const int64_t stride_k[3], const int64_t stride_v[3], int dtype);
+
+/* Attention of one token per sequence over the cache: q, o [batch, Hq, D] of `dtype` (F16 or BF16, strides
+ * {sequence, head, d}, multiples of 8 but for d), over the first seq_lens[b] tokens of sequence b (cut at
+ * max_pages * page_size).  m (may be NULL): [batch, Hq] fp32, base-2 log-sum-exp.  A sequence without tokens
+ * gives zeros and -inf.  `workspace`: b200_attention_decode_workspace(...) bytes (0: none needed), 16-byte
+ * aligned, the caller's scratch for the call; calls that may overlap need one each.  Bitwise repeatable. */
+B200_API size_t b200_attention_decode_workspace(int batch, int Hq, int Hkv, int D, int page_size, int max_pages);
+B200_API int b200_attention_decode(b200_stream_t stream, const void* q, const void* k_cache, const void* v_cache,
+                                   const float* k_scale, const float* v_scale, int pages, int page_size,
+                                   const int* page_table, int64_t table_stride, int max_pages, const int* seq_lens,
+                                   void* o, float* m, int batch, int Hq, int Hkv, int D, const int64_t stride_q[3],
+                                   const int64_t stride_o[3], float sm_scale, int dtype, void* workspace);
+
 #ifdef __cplusplus
 }
 #endif

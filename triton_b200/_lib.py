@@ -17,6 +17,7 @@ BIAS_NONE, BIAS_MATRIX, BIAS_ROWS, BIAS_COLS = 0, 1, 2, 3
 
 _i, _i64, _p, _f = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float
 _s4 = ctypes.c_int64 * 4  # an element-stride quadruple {z, h, n, d}
+_s3 = ctypes.c_int64 * 3  # {token or sequence, h, d}
 
 # name -> argument types; every function returns int except where noted below
 SIGNATURES = {
@@ -43,6 +44,10 @@ SIGNATURES = {
     "b200_attention_bwd_wide_workspace": [_i],
     "b200_attention_bwd_noalloc": [_p] + [_p] * 9 + [_i, _i, _i, _i] + [_s4] * 8 + [_f, _i, _i],
     "b200_attention_bwd_noalloc_capacity": [],
+    "b200_attention_varlen_fwd": [_p] * 7 + [_i] * 5 + [_s3] * 4 + [_f, _i, _i, _i],
+    "b200_kv_append": [_p] * 5 + [_i, _i, _p, _i64, _i, _p, _p, _p, _p, _i, _i, _i, _i, _s3, _s3, _i],
+    "b200_attention_decode_workspace": [_i] * 6,
+    "b200_attention_decode": [_p] * 6 + [_i, _i, _p, _i64, _i, _p, _p, _p, _i, _i, _i, _i, _s3, _s3, _f, _i, _p],
 }
 
 _lib = None
@@ -80,6 +85,10 @@ def check(code, what):
 
 def strides4(t):
     return _s4(*t.stride())
+
+
+def strides3(t):
+    return _s3(*t.stride())
 
 
 def status(clear=True):

@@ -1,0 +1,57 @@
+// Attention over packed prompts with grouped heads: tensor maps and launches of the packed form of the
+// kernel in attn_fwd_kernel.cuh.
+#include "attn_fwd_kernel.cuh"
+#include "serving.h"
+
+namespace tb {
+
+namespace {
+
+template <int D, bool BF16>
+int launch_packed_t(DeviceCtx* ctx, cudaStream_t stream, const CUtensorMap& tq, const CUtensorMap& tk,
+                    const CUtensorMap& tv, const CUtensorMap& to, const PackedFwdParams& p, long long most_items) {
+  static std::atomic<bool> attr_done[64];
+  constexpr size_t smem = FwdCfg<D>::SMEM + 64;  // + the published items
+  if (int rc = ensure_dynamic_smem(attn_fwd_kernel<D, BF16, false, true>, smem, ctx->device, attr_done, "attn varlen")) return rc;
+  const int grid = most_items < 1 ? 1 : (most_items < ctx->sm_count ? (int)most_items : ctx->sm_count);
+  attn_fwd_kernel<D, BF16, false, true><<<grid, FWD_THREADS, smem, stream>>>(tq, tk, tv, to, p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return fail(B200_ERR_CUDA, "attn varlen launch: %s", cudaGetErrorString(e));
+  return B200_OK;
+}
+
+}  // namespace
+
+int launch_attn_varlen(DeviceCtx* ctx, cudaStream_t stream, const AttnVarlenArgs& a) {
+  CUtensorMap tq, tk, tv, to;
+  if (!encode_qkv_map(&tq, a.dtype, a.q, 1, a.Hq, a.T, a.D, 0, a.sq[1], a.sq[0], BLK)) return B200_ERR_UNSUPPORTED;
+  if (!encode_qkv_map(&tk, a.dtype, a.k, 1, a.Hkv, a.T, a.D, 0, a.sk[1], a.sk[0], BLK)) return B200_ERR_UNSUPPORTED;
+  if (!encode_qkv_map(&tv, a.dtype, a.v, 1, a.Hkv, a.T, a.D, 0, a.sv[1], a.sv[0], BLK)) return B200_ERR_UNSUPPORTED;
+  if (!encode_qkv_map(&to, a.dtype, a.o, 1, a.Hq, a.T, a.D, 0, a.so[1], a.so[0], 32)) return B200_ERR_UNSUPPORTED;
+  PackedFwdParams p{};
+  p.o_tma = 1;
+  p.o = a.o;
+  p.m = a.m;
+  p.o_sh = a.so[1];
+  p.o_sn = a.so[0];
+  p.Z = 1;
+  p.H = a.Hq;
+  p.N = a.T;
+  p.causal = a.causal;
+  p.scale_log2 = a.sm_scale * 1.44269504f;
+  p.cu = a.cu;
+  p.batch = a.batch;
+  p.group = a.Hq / a.Hkv;
+  p.zero_rest = a.zero_rest;
+  p.status = ctx->status;
+  p.sched_counter = next_sched_counter(ctx, stream);
+  if (!p.sched_counter) return B200_ERR_CUDA;
+  const int item_rows = (a.D == 256) ? BLK : 2 * BLK;
+  const long long most_items = ((long long)a.T / item_rows + a.batch) * a.Hq;  // the lengths are on the device
+  const bool bf16 = a.dtype == B200_BF16;
+  if (a.D == 256) return bf16 ? launch_packed_t<256, true>(ctx, stream, tq, tk, tv, to, p, most_items) : launch_packed_t<256, false>(ctx, stream, tq, tk, tv, to, p, most_items);
+  if (a.D == 128) return bf16 ? launch_packed_t<128, true>(ctx, stream, tq, tk, tv, to, p, most_items) : launch_packed_t<128, false>(ctx, stream, tq, tk, tv, to, p, most_items);
+  return bf16 ? launch_packed_t<64, true>(ctx, stream, tq, tk, tv, to, p, most_items) : launch_packed_t<64, false>(ctx, stream, tq, tk, tv, to, p, most_items);
+}
+
+}  // namespace tb

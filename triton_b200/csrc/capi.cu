@@ -7,6 +7,7 @@
 
 #include "common.cuh"
 #include "host.h"
+#include "serving.h"
 
 namespace tb {
 
@@ -617,6 +618,133 @@ int b200_attention_bwd_noalloc(b200_stream_t stream, const void* q, const void* 
   // same validation and launches as the caller-scratch entry point, on the built-in array
   return b200_attention_bwd(stream, q, k, v, o, d_o, m, delta, dq, dk, dv, Z, H, N, D, stride_q, stride_k, stride_v,
                             stride_o, stride_do, stride_dq, stride_dk, stride_dv, sm_scale, causal, dtype);
+}
+
+int b200_attention_varlen_fwd(b200_stream_t stream, const void* q, const void* k, const void* v, void* o, float* m,
+                              const int* cu_seqlens, int batch, int T, int Hq, int Hkv, int D, const int64_t stride_q[3],
+                              const int64_t stride_k[3], const int64_t stride_v[3], const int64_t stride_o[3],
+                              float sm_scale, int causal, int dtype, int zero_rest) {
+  if (batch < 0 || T < 0 || Hq < 0 || Hkv < 0) return fail(B200_ERR_ARG, "negative dimension");
+  if (dtype != B200_F16 && dtype != B200_BF16) return fail(B200_ERR_ARG, "attention dtype must be F16 or BF16");
+  if (D != 64 && D != 128 && D != 256)
+    return fail(B200_ERR_UNSUPPORTED, "head dim %d: the forward has kernels for 64, 128 and 256", D);
+  if (Hkv == 0 ? Hq != 0 : Hq % Hkv != 0) return fail(B200_ERR_ARG, "%d query heads are no multiple of %d k/v heads", Hq, Hkv);
+  if (!(sm_scale > 0.f)) return fail(B200_ERR_ARG, "sm_scale must be positive");
+  const int64_t* all[4] = {stride_q, stride_k, stride_v, stride_o};
+  for (const int64_t* st : all) {
+    if (!st) return fail(B200_ERR_ARG, "null stride array");
+    if (st[2] != 1) return fail(B200_ERR_UNSUPPORTED, "the head dimension must be contiguous");
+  }
+  if (((long long)T / 128 + batch + 1) * Hq > 0x3fffffffLL) return fail(B200_ERR_UNSUPPORTED, "too many work items");
+  DeviceCtx* ctx = ready_ctx();
+  if (!ctx) return g_err_code;
+  if (T == 0 || Hq == 0 || (batch == 0 && !zero_rest)) return B200_OK;
+  if (!q || !k || !v || !o || !cu_seqlens) return fail(B200_ERR_ARG, "null pointer");
+  AttnVarlenArgs a{};
+  a.q = q; a.k = k; a.v = v; a.o = o; a.m = m; a.cu = cu_seqlens;
+  a.batch = batch; a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.D = D;
+  for (int i = 0; i < 2; ++i) { a.sq[i] = stride_q[i]; a.sk[i] = stride_k[i]; a.sv[i] = stride_v[i]; a.so[i] = stride_o[i]; }
+  a.sm_scale = sm_scale; a.causal = causal ? 1 : 0; a.dtype = dtype; a.zero_rest = zero_rest ? 1 : 0;
+  return launch_attn_varlen(ctx, reinterpret_cast<cudaStream_t>(stream), a);
+}
+
+// what the two entry points on a paged cache have in common
+static int paged_cache_args(PagedCache* c, const void* k_cache, const void* v_cache, const float* k_scale,
+                            const float* v_scale, const int* page_table, int64_t table_stride, int pages, int page_size,
+                            int max_pages, int Hkv, int D) {
+  if (pages < 0 || max_pages < 0 || Hkv < 0) return fail(B200_ERR_ARG, "negative dimension");
+  if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128)
+    return fail(B200_ERR_UNSUPPORTED, "page size %d: pages hold 16, 32, 64 or 128 tokens", page_size);
+  if (D != 64 && D != 128 && D != 256) return fail(B200_ERR_UNSUPPORTED, "head dim %d: a cache has head dim 64, 128 or 256", D);
+  if ((long long)max_pages * page_size > 0x7fffffffLL - 128) return fail(B200_ERR_UNSUPPORTED, "page table too wide");
+  if ((long long)pages * Hkv * (page_size / 16) >= 0xffffffffLL || Hkv > 65535)
+    return fail(B200_ERR_UNSUPPORTED, "cache too large");
+  c->k = static_cast<uint8_t*>(const_cast<void*>(k_cache));
+  c->v = static_cast<uint8_t*>(const_cast<void*>(v_cache));
+  c->k_scale = const_cast<float*>(k_scale);
+  c->v_scale = const_cast<float*>(v_scale);
+  c->table = page_table;
+  c->table_stride = table_stride;
+  c->pages = pages; c->page_size = page_size; c->max_pages = max_pages; c->Hkv = Hkv; c->D = D;
+  if ((reinterpret_cast<uintptr_t>(k_cache) & 15) || (reinterpret_cast<uintptr_t>(v_cache) & 15))
+    return fail(B200_ERR_UNSUPPORTED, "the cache must be 16-byte aligned");
+  return B200_OK;
+}
+
+int b200_kv_append(b200_stream_t stream, void* k_cache, void* v_cache, float* k_scale, float* v_scale, int pages,
+                   int page_size, const int* page_table, int64_t table_stride, int max_pages, const int* seq_lens,
+                   const void* k, const void* v, const int* cu_seqlens, int batch, int T, int Hkv, int D,
+                   const int64_t stride_k[3], const int64_t stride_v[3], int dtype) {
+  if (batch < 0 || T < 0) return fail(B200_ERR_ARG, "negative dimension");
+  if (dtype != B200_F16 && dtype != B200_BF16) return fail(B200_ERR_ARG, "new rows must be F16 or BF16");
+  KvAppendArgs a{};
+  if (int rc = paged_cache_args(&a.c, k_cache, v_cache, k_scale, v_scale, page_table, table_stride, pages, page_size,
+                                max_pages, Hkv, D))
+    return rc;
+  if (!cu_seqlens && T != batch) return fail(B200_ERR_ARG, "without cu_seqlens every sequence has one new row (T == batch)");
+  const int64_t* all[2] = {stride_k, stride_v};
+  for (const int64_t* st : all) {
+    if (!st) return fail(B200_ERR_ARG, "null stride array");
+    if (st[2] != 1) return fail(B200_ERR_UNSUPPORTED, "the head dimension must be contiguous");
+    if ((T > 1 && (st[0] & 7)) || (Hkv > 1 && (st[1] & 7))) return fail(B200_ERR_UNSUPPORTED, "strides must be multiples of 8 elements");
+  }
+  if ((reinterpret_cast<uintptr_t>(k) & 15) || (reinterpret_cast<uintptr_t>(v) & 15))
+    return fail(B200_ERR_UNSUPPORTED, "new rows must be 16-byte aligned");
+  if ((long long)T / page_size + 2LL * batch > 0x7fffffffLL || (long long)batch * Hkv > 0x3fffffffLL)
+    return fail(B200_ERR_UNSUPPORTED, "too many work items");
+  DeviceCtx* ctx = ready_ctx();
+  if (!ctx) return g_err_code;
+  if (T == 0 || batch == 0 || Hkv == 0 || pages == 0 || max_pages == 0) return B200_OK;
+  if (!k_cache || !v_cache || !k_scale || !v_scale || !page_table || !seq_lens || !k || !v)
+    return fail(B200_ERR_ARG, "null pointer");
+  a.k = k; a.v = v;
+  a.k_st = stride_k[0]; a.k_sh = stride_k[1]; a.v_st = stride_v[0]; a.v_sh = stride_v[1];
+  a.lens = seq_lens; a.cu = cu_seqlens;
+  a.batch = batch; a.T = T; a.dtype = dtype;
+  return launch_kv_append(ctx, reinterpret_cast<cudaStream_t>(stream), a);
+}
+
+size_t b200_attention_decode_workspace(int batch, int Hq, int Hkv, int D, int page_size, int max_pages) {
+  if (batch <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || page_size < 16 || max_pages <= 0) return 0;
+  return attn_decode_workspace_bytes(batch, Hq, Hkv, D, page_size, max_pages);
+}
+
+int b200_attention_decode(b200_stream_t stream, const void* q, const void* k_cache, const void* v_cache,
+                          const float* k_scale, const float* v_scale, int pages, int page_size, const int* page_table,
+                          int64_t table_stride, int max_pages, const int* seq_lens, void* o, float* m, int batch, int Hq,
+                          int Hkv, int D, const int64_t stride_q[3], const int64_t stride_o[3], float sm_scale, int dtype,
+                          void* workspace) {
+  if (batch < 0 || Hq < 0) return fail(B200_ERR_ARG, "negative dimension");
+  if (dtype != B200_F16 && dtype != B200_BF16) return fail(B200_ERR_ARG, "attention dtype must be F16 or BF16");
+  AttnDecodeArgs a{};
+  if (int rc = paged_cache_args(&a.c, k_cache, v_cache, k_scale, v_scale, page_table, table_stride, pages, page_size,
+                                max_pages, Hkv, D))
+    return rc;
+  if (Hkv == 0 ? Hq != 0 : Hq % Hkv != 0) return fail(B200_ERR_ARG, "%d query heads are no multiple of %d k/v heads", Hq, Hkv);
+  if (!(sm_scale > 0.f)) return fail(B200_ERR_ARG, "sm_scale must be positive");
+  const int64_t* all[2] = {stride_q, stride_o};
+  for (const int64_t* st : all) {
+    if (!st) return fail(B200_ERR_ARG, "null stride array");
+    if (st[2] != 1) return fail(B200_ERR_UNSUPPORTED, "the head dimension must be contiguous");
+    if ((batch > 1 && (st[0] & 7)) || (Hq > 1 && (st[1] & 7))) return fail(B200_ERR_UNSUPPORTED, "strides must be multiples of 8 elements");
+  }
+  if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(o) & 15))
+    return fail(B200_ERR_UNSUPPORTED, "q and o must be 16-byte aligned");
+  if (batch > 65535 || Hq > 65535) return fail(B200_ERR_UNSUPPORTED, "at most 65535 sequences and heads in a call");
+  DeviceCtx* ctx = ready_ctx();
+  if (!ctx) return g_err_code;
+  if (batch == 0 || Hq == 0) return B200_OK;
+  if (!q || !o || !seq_lens || (pages > 0 && max_pages > 0 && (!k_cache || !v_cache || !k_scale || !v_scale || !page_table)))
+    return fail(B200_ERR_ARG, "null pointer");
+  if (b200_attention_decode_workspace(batch, Hq, Hkv, D, page_size, max_pages) > 0 &&
+      (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+    return fail(B200_ERR_ARG, "needs a 16-byte aligned workspace of b200_attention_decode_workspace(...) bytes");
+  if (pages == 0) a.c.max_pages = 0;  // no page to name: every sequence is empty
+  a.q = q; a.o = o; a.m = m;
+  a.q_sb = stride_q[0]; a.q_sh = stride_q[1]; a.o_sb = stride_o[0]; a.o_sh = stride_o[1];
+  a.lens = seq_lens; a.B = batch; a.Hq = Hq; a.sm_scale = sm_scale; a.dtype = dtype;
+  a.workspace = static_cast<float*>(workspace);
+  return launch_attn_decode(ctx, reinterpret_cast<cudaStream_t>(stream), a);
 }
 
 }  // extern "C"

@@ -1,10 +1,10 @@
 """PyTorch custom-op registration of the library's entry points.
 
-`torch.ops.triton_b200.matmul`, `.attention_fwd`, `.attention_bwd` and the differentiable
-`.attention` are registered with `torch.library.custom_op`: they show up in the dispatcher, have
+`torch.ops.triton_b200.matmul`, `.attention_fwd`, `.attention_bwd`, the differentiable `.attention` and the
+serving calls `.attention_varlen`, `.kv_cache_append` (in place) and `.attention_decode` are registered with `torch.library.custom_op`: they show up in the dispatcher, have
 fake (meta) implementations so that `torch.compile` / export can trace through them without
 running a kernel, and `attention` carries its backward formula.  The CUDA implementations are the
-functions of `triton_b200.ops`, i.e. the C ABI of include/triton_b200.h through ctypes; there is
+functions of `triton_b200.ops` and `triton_b200.serving`, i.e. the C ABI of include/triton_b200.h through ctypes; there is
 no CPU implementation: on CPU tensors the ops raise, like the functions they wrap.
 """
 from typing import Optional, Tuple
@@ -12,7 +12,7 @@ from typing import Optional, Tuple
 import torch
 from torch import Tensor
 
-from . import ops
+from . import ops, serving
 
 _lib_ns = "triton_b200"
 
@@ -78,3 +78,36 @@ def _attention_backward(ctx, do, dM):
 
 
 torch.library.register_autograd(f"{_lib_ns}::attention", _attention_backward, setup_context=_attention_setup)
+
+
+@torch.library.custom_op(f"{_lib_ns}::attention_varlen", mutates_args=(), device_types="cuda")
+def attention_varlen(q: Tensor, k: Tensor, v: Tensor, cu_seqlens: Tensor, causal: bool, sm_scale: float) -> Tensor:
+    return serving.attention_varlen(q, k, v, cu_seqlens, causal, sm_scale)
+
+
+@attention_varlen.register_fake
+def _(q, k, v, cu_seqlens, causal, sm_scale):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op(f"{_lib_ns}::kv_cache_append", mutates_args=("k_cache", "v_cache", "k_scale", "v_scale"),
+                         device_types="cuda")
+def kv_cache_append(k_cache: Tensor, v_cache: Tensor, k_scale: Tensor, v_scale: Tensor, k: Tensor, v: Tensor,
+                    page_table: Tensor, seq_lens: Tensor, cu_seqlens: Optional[Tensor] = None) -> None:
+    serving.kv_cache_append(k_cache, v_cache, k_scale, v_scale, k, v, page_table, seq_lens, cu_seqlens)
+
+
+@kv_cache_append.register_fake
+def _(k_cache, v_cache, k_scale, v_scale, k, v, page_table, seq_lens, cu_seqlens=None):
+    return None
+
+
+@torch.library.custom_op(f"{_lib_ns}::attention_decode", mutates_args=(), device_types="cuda")
+def attention_decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_scale: Tensor, v_scale: Tensor, page_table: Tensor,
+                     seq_lens: Tensor, sm_scale: float) -> Tensor:
+    return serving.attention_decode(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, sm_scale)
+
+
+@attention_decode.register_fake
+def _(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, sm_scale):
+    return q.new_empty(q.shape)
