@@ -8,8 +8,10 @@
 // products run on warp-level MMAs (m16n8k16, fp32 accumulators) with the cache as the 16-row operand:
 //   S^T = K Q^T   (16 tokens x 8 query heads),   O^T += V^T P^T   (16 head-dim indices x 8 query heads).
 // A head dimension is a contraction in any order and tokens may take any slot, so each lane loads 16
-// consecutive bytes of a row straight from global memory into the operand's registers: no shared memory,
-// no transposes of K or V (P^T is turned by two 8 x 8 register transposes).  e4m3 -> fp16 is exact.
+// consecutive bytes of a row into the operand's registers: no transposes of K or V (P^T is turned by two
+// 8 x 8 register transposes).  e4m3 -> fp16 is exact.  Each warp fetches its slabs through a ring of its own in
+// shared memory (cp.async), 8 to 10 KB ahead: with loads straight to registers, 4 KB ahead, 131000 tokens of
+// 8 heads x 128 took 94 us.
 //
 // Roundings to 16 bits: q in fp16 as it is, in bf16 times a power of two of its row that brings the row's
 // largest value near fp16's top (8 significant bits fit; what lies 2^-29 below the largest loses bits);
@@ -29,7 +31,7 @@ namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int SLAB = 16;             // tokens of one MMA
-constexpr int MAX_CHUNK_SLABS = 1024;  // page-table entries a CTA keeps in shared memory
+constexpr int MAX_CHUNK_SLABS = 256;  // page-table entries a CTA keeps in shared memory
 constexpr float REF_NONE = -1.7e38f;   // reference point before the first token: finite, below every score
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -47,10 +49,10 @@ DecodePlan decode_plan(int B, int Hq, int Hkv, int D, int page_size, int max_pag
   p.row_blocks = (G + 8 * p.nt - 1) / (8 * p.nt);
   const long long slabs = (long long)max_pages * (page_size / SLAB);
   const long long ctas = (long long)B * Hkv * p.row_blocks;
-  const long long want = 148 * 8;
+  const long long want = 148 * 6;
   long long splits = (want + ctas - 1) / ctas;
   long long chunk = (slabs + splits - 1) / splits;
-  if (chunk < 16) chunk = 16;
+  if (chunk < 8) chunk = 8;
   if (chunk > MAX_CHUNK_SLABS) chunk = MAX_CHUNK_SLABS;
   p.chunk = (int)chunk;
   p.splits = (int)((slabs + chunk - 1) / chunk);
@@ -76,6 +78,11 @@ struct DecodeParams {
   float* ws_lse;  // [B, Hq, splits] their base-2 log-sum-exp
 };
 
+// A warp takes STEP slabs at once (two: independent chains of MMAs) and owns a ring of two such steps in
+// shared memory, K and V refilled as soon as each has been read.
+template <int D> constexpr int STEP = D == 256 ? 1 : 2;
+template <int D> constexpr int RING = 2 * STEP<D> * SLAB * D * 2;
+
 struct SlabEntry {
   unsigned slab;  // index of 16-token slabs in the cache (times 16 * D bytes); ~0u: no page
   float ks;
@@ -98,76 +105,81 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ uint4 ldg_stream(const uint8_t* p) {  // read once: no room in L1
-  uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
-  return r;
-}
-__device__ __forceinline__ uint2 ldg_stream8(const uint8_t* p) {
-  uint2 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
-  return r;
-}
-
-// One slab's bytes in registers.  K: words of rows g and g + 8 (g = lane / 4), for each 64-byte part of the
-// row the 16 bytes at 16 * (lane % 4).  V: of tokens 2c, 2c + 1, 2c + 8, 2c + 9 (c = lane % 4) the D / 8
-// bytes at (D / 8) * g.
+// One slab (16 tokens of K, then of V) in shared memory: rows of D bytes, the 16-byte parts of a row XORed
+// with bits of the row so that the loads below meet no bank twice (V at head dim 64: twice).
 template <int D>
-struct SlabRegs {
-  uint32_t k[2][D / 16];
-  uint32_t v[4][D / 32];
-};
+__device__ __forceinline__ uint32_t part_offset(int row, int part) {
+  if constexpr (D == 64) return row * 64 + ((part ^ ((row >> 1) & 3)) << 4);
+  else return row * D + ((part ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const uint8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// one slab's K or V into shared memory: consecutive lanes, consecutive 16 bytes
 template <int D>
-__device__ __forceinline__ void load_slab(SlabRegs<D>& r, const DecodeParams& p, unsigned slab, int g, int c) {
-  const unsigned long long at = (unsigned long long)slab * (SLAB * D);
-  const uint8_t* kp = p.k + at + g * D + c * 16;
+__device__ __forceinline__ void fetch_slab(uint32_t dst, const uint8_t* src, unsigned slab, int lane) {
+  src += (unsigned long long)slab * (SLAB * D) + lane * 16;
 #pragma unroll
-  for (int part = 0; part < D / 64; ++part) {
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const uint4 x = ldg_stream(kp + half * 8 * D + part * 64);
-      r.k[half][4 * part] = x.x; r.k[half][4 * part + 1] = x.y; r.k[half][4 * part + 2] = x.z; r.k[half][4 * part + 3] = x.w;
-    }
+  for (int i = 0; i < D / 32; ++i) {
+    const int q = i * 32 + lane;
+    cp_async16(dst + part_offset<D>(q / (D / 16), q % (D / 16)), src + i * 512);
   }
-  const uint8_t* vp = p.v + at + g * (D / 8);
+}
+
+// head-dim index of K's word w for lane c, and of V's byte pair i for lane g
+template <int D>
+__device__ __forceinline__ int k_index(int c, int w) { return (w >> 3) * 128 + c * (D == 64 ? 16 : 32) + (w & 7) * 4; }
+template <int D>
+__device__ __forceinline__ int v_index(int g, int i) { return (i >> 3) * 128 + g * (D == 64 ? 8 : 16) + (i & 7) * 2; }
+
+// K in registers: rows g and g + 8 (g = lane / 4); of every 128 bytes of the row (or the 64 of head dim 64) the
+// quarter of c = lane % 4.
+template <int D>
+__device__ __forceinline__ void read_k(uint32_t (&k)[2][D / 16], const uint8_t* at, int g, int c) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint8_t* row = vp + (2 * c + (i & 1) + (i >> 1) * 8) * D;
+  for (int half = 0; half < 2; ++half)
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+      const int part = (D == 64) ? c : (i >> 1) * 8 + 2 * c + (i & 1);
+      const uint4 x = *reinterpret_cast<const uint4*>(at + part_offset<D>(g + 8 * half, part));
+      k[half][4 * i] = x.x; k[half][4 * i + 1] = x.y; k[half][4 * i + 2] = x.z; k[half][4 * i + 3] = x.w;
+    }
+}
+// V in registers: of tokens 2c, 2c + 1, 2c + 8, 2c + 9 the D / 8 bytes of g, at head dim 256 16 in each half of the row
+template <int D>
+__device__ __forceinline__ void read_v(uint32_t (&v)[4][D / 32], const uint8_t* at, int g, int c) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const int row = 2 * c + (t & 1) + (t >> 1) * 8;
     if constexpr (D == 64) {
-      const uint2 x = ldg_stream8(row);
-      r.v[i][0] = x.x; r.v[i][1] = x.y;
+      const uint2 x = *reinterpret_cast<const uint2*>(at + part_offset<D>(row, g >> 1) + (g & 1) * 8);
+      v[t][0] = x.x; v[t][1] = x.y;
     } else {
 #pragma unroll
-      for (int part = 0; part < D / 128; ++part) {
-        const uint4 x = ldg_stream(row + part * 16);
-        r.v[i][4 * part] = x.x; r.v[i][4 * part + 1] = x.y; r.v[i][4 * part + 2] = x.z; r.v[i][4 * part + 3] = x.w;
+      for (int i = 0; i < D / 128; ++i) {
+        const uint4 x = *reinterpret_cast<const uint4*>(at + part_offset<D>(row, i * 8 + g));
+        v[t][4 * i] = x.x; v[t][4 * i + 1] = x.y; v[t][4 * i + 2] = x.z; v[t][4 * i + 3] = x.w;
       }
     }
   }
 }
 
-template <bool BF16>
-__device__ __forceinline__ float to_f32(uint16_t x) {
-  if constexpr (BF16) return __uint_as_float((uint32_t)x << 16);
-  else return __half2float(__ushort_as_half(x));
-}
-template <bool BF16>
-__device__ __forceinline__ uint16_t from_f32(float x) {
-  if constexpr (BF16) return __bfloat16_as_ushort(__float2bfloat16_rn(x));
-  else return __half_as_ushort(__float2half_rn(x));
-}
-
 template <int D, int NT, bool BF16>
-__global__ void __launch_bounds__(THREADS) attn_decode_kernel(const DecodeParams p) {
+__global__ void __launch_bounds__(THREADS, 3) attn_decode_kernel(const DecodeParams p) {
   constexpr int ROWS = 8 * NT, KSTEPS = D / 16, MT = D / 16;
   constexpr int OSTRIDE = D + 4;  // floats; + 4 spreads the rows over the banks
-  extern __shared__ __align__(16) uint8_t smem[];
-  SlabEntry* table = reinterpret_cast<SlabEntry*>(smem);                          // [chunk]
+  constexpr int SL = STEP<D>, SIDE = SLAB * D, STAGE = 2 * SL * SIDE;  // a stage: SL slabs of K, then of V
+  extern __shared__ __align__(128) uint8_t smem[];  // [WARPS] rings, then the chunk's page entries
+  SlabEntry* table = reinterpret_cast<SlabEntry*>(smem + WARPS * RING<D>);
   __shared__ float s_refw[WARPS][ROWS], s_refp[WARPS][ROWS], s_l[WARPS][ROWS];
   __shared__ int s_seen[WARPS];
-  float* so = reinterpret_cast<float*>(smem);                                     // [WARPS][ROWS][OSTRIDE], after the loop
+  float* so = reinterpret_cast<float*>(smem);                                     // [WARPS][ROWS][OSTRIDE], over the rings after the loop
 
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (without a dependent kernel: nothing)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int split = blockIdx.x, b = blockIdx.z;
   const int h = blockIdx.y / p.row_blocks, rb = blockIdx.y % p.row_blocks;
@@ -193,7 +205,7 @@ __global__ void __launch_bounds__(THREADS) attn_decode_kernel(const DecodeParams
     table[i] = e;
   }
 
-  // q as the B operand: for the 64-byte part and word of k-step s, the four head-dim indices of that word
+  // q as the B operand: for k-step s the four head-dim indices of K's word s
   uint32_t qf[KSTEPS][NT][2];
   float fac[NT][2];  // per query row 2c, 2c + 1 of each group: score of one unit of the product, log2 units
 #pragma unroll
@@ -203,7 +215,7 @@ __global__ void __launch_bounds__(THREADS) attn_decode_kernel(const DecodeParams
     uint2 raw[KSTEPS];
 #pragma unroll
     for (int s = 0; s < KSTEPS; ++s) {
-      raw[s] = __ldg(reinterpret_cast<const uint2*>(qr + (s >> 2) * 64 + c * 16 + (s & 3) * 4));
+      raw[s] = __ldg(reinterpret_cast<const uint2*>(qr + k_index<D>(c, s)));
       if (row >= nrows) raw[s] = make_uint2(0, 0);
     }
     float f = p.sm_scale_log2;
@@ -251,64 +263,110 @@ __global__ void __launch_bounds__(THREADS) attn_decode_kernel(const DecodeParams
 
   __syncthreads();
   const int count = s1 - s0;
-  SlabRegs<D> cur, nxt;
-  if (warp < count && table[warp].slab != ~0u) load_slab<D>(cur, p, table[warp].slab, g, c);
-  for (int i = warp; i < count; i += WARPS) {
-    const SlabEntry e = table[i];
-    if (i + WARPS < count && table[i + WARPS].slab != ~0u) load_slab<D>(nxt, p, table[i + WARPS].slab, g, c);
-    if (e.slab != ~0u) {
-      seen = 1;
-      float s[NT][4];
+  uint8_t* ring = smem + warp * RING<D>;
+  auto fetch = [&](int i, int st, int side) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+    for (int u = 0; u < SL; ++u)
+      if (i + u < count && table[i + u].slab != ~0u)
+        fetch_slab<D>(smem_u32(ring) + st * STAGE + (side * SL + u) * SIDE, side ? p.v : p.k, table[i + u].slab, lane);
+    cp_async_commit();
+  };
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[t][j] = 0.f;
+  for (int st = 0; st < 2; ++st) {
+    fetch((st * WARPS + warp) * SL, st, 0);
+    fetch((st * WARPS + warp) * SL, st, 1);
+  }
+  int st = 0;
+  for (int i = warp * SL; i < count; i += WARPS * SL, st ^= 1) {
+    const uint8_t* stage = ring + st * STAGE;
+    const int next = i + 2 * WARPS * SL;
+    float ks[SL], ev[SL];
+    int left[SL];  // tokens of the slab that exist
+    bool any_here = false;
 #pragma unroll
-      for (int k = 0; k < KSTEPS; ++k) {
-        const uint32_t x = cur.k[0][k], y = cur.k[1][k];
-        const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)x), a1 = e4m3x2_to_f16x2((uint16_t)y);
-        const uint32_t a2 = e4m3x2_to_f16x2((uint16_t)(x >> 16)), a3 = e4m3x2_to_f16x2((uint16_t)(y >> 16));
+    for (int u = 0; u < SL; ++u) {
+      SlabEntry e{~0u, 0.f, 0.f};
+      if (u == 0 || i + u < count) e = table[i + u];
+      ks[u] = e.ks;
+      ev[u] = e.ev;
+      left[u] = e.slab != ~0u ? len - (s0 + i + u) * SLAB : 0;
+      any_here |= e.slab != ~0u;
+    }
+    // groups were committed in the order K, V of this step, K, V of the next; each wait leaves three
+    float s[SL][NT][4];
+    cp_async_wait<3>();
+    __syncwarp();
+    if (any_here) {
+      uint32_t kr[SL][2][D / 16];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) mma_f16(s[t], a0, a1, a2, a3, qf[k][t][0], qf[k][t][1]);
-      }
-      // scores in log2 units; columns behind the last token vanish, and so do V's rows there (their bytes
-      // are whatever an earlier owner of the page left)
-      const int left = len - (s0 + i) * SLAB;
+      for (int u = 0; u < SL; ++u) read_k<D>(kr[u], stage + u * SIDE, g, c);
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[t][j] = (s[t][j] * fac[t][j & 1]) * e.ks;
-      if (left < SLAB) {
+      for (int u = 0; u < SL; ++u)
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (g + (j >> 1) * 8 >= left) s[t][j] = -INFINITY;
+          for (int j = 0; j < 4; ++j) s[u][t][j] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (2 * c + (j & 1) + (j >> 1) * 8 >= left) {
+      for (int k = 0; k < KSTEPS; ++k)
 #pragma unroll
-            for (int k = 0; k < D / 32; ++k) cur.v[j][k] = 0u;
-          }
+        for (int u = 0; u < SL; ++u) {
+          const uint32_t x = kr[u][0][k], y = kr[u][1][k];
+          const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)x), a1 = e4m3x2_to_f16x2((uint16_t)y);
+          const uint32_t a2 = e4m3x2_to_f16x2((uint16_t)(x >> 16)), a3 = e4m3x2_to_f16x2((uint16_t)(y >> 16));
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma_f16(s[u][t], a0, a1, a2, a3, qf[k][t][0], qf[k][t][1]);
+        }
+    }
+    __syncwarp();
+    fetch(next, st, 0);
+    uint32_t pb[SL][NT][2];
+    if (any_here) {
+      seen = 1;
+      // scores in log2 units; those behind the last token and of pages that do not exist vanish
+#pragma unroll
+      for (int u = 0; u < SL; ++u) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[u][t][j] = (s[u][t][j] * fac[t][j & 1]) * ks[u];
+        if (left[u] < SLAB) {
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (g + (j >> 1) * 8 >= left[u]) s[u][t][j] = -INFINITY;
+        }
       }
       // new reference points where a weight would pass 2^15 (numerators) or 2^40 (denominator)
+      float topw[NT][2], topp[NT][2];
       bool grow = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const float top = fmaxf(s[t][j], s[t][j + 2]);
-          grow |= (top + e.ev - refw[t][j] > 15.f) || (top - refp[t][j] > 40.f);
+          float a = fmaxf(s[0][t][j], s[0][t][j + 2]);
+          topp[t][j] = a;
+          topw[t][j] = a + ev[0];
+#pragma unroll
+          for (int u = 1; u < SL; ++u) {
+            a = fmaxf(s[u][t][j], s[u][t][j + 2]);
+            topp[t][j] = fmaxf(topp[t][j], a);
+            topw[t][j] = fmaxf(topw[t][j], a + ev[u]);
+          }
+          grow |= (topw[t][j] - refw[t][j] > 15.f) || (topp[t][j] - refp[t][j] > 40.f);
         }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float top = fmaxf(s[t][j], s[t][j + 2]);
+            float tw = topw[t][j], tp = topp[t][j];
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-            const float w = fmaxf(refw[t][j], top + e.ev - 7.f), q = fmaxf(refp[t][j], top);
+            for (int x = 4; x < 32; x <<= 1) {
+              tw = fmaxf(tw, __shfl_xor_sync(0xffffffffu, tw, x));
+              tp = fmaxf(tp, __shfl_xor_sync(0xffffffffu, tp, x));
+            }
+            const float w = fmaxf(refw[t][j], tw - 7.f), q = fmaxf(refp[t][j], tp);
             const float alpha = ex2(refw[t][j] - w);
             l[t][j] *= ex2(refp[t][j] - q);
             refw[t][j] = w;
@@ -317,31 +375,51 @@ __global__ void __launch_bounds__(THREADS) attn_decode_kernel(const DecodeParams
             for (int k = 0; k < MT; ++k) { o[k][t][j] *= alpha; o[k][t][j + 2] *= alpha; }
           }
       }
-      uint32_t pb[NT][2];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float w[4];
+      for (int u = 0; u < SL; ++u)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          w[j] = ex2(s[t][j] + e.ev - refw[t][j & 1]);
-          l[t][j & 1] += ex2(s[t][j] - refp[t][j & 1]);
+        for (int t = 0; t < NT; ++t) {
+          float w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            w[j] = ex2(s[u][t][j] + (ev[u] - refw[t][j & 1]));
+            l[t][j & 1] += ex2(s[u][t][j] - refp[t][j & 1]);
+          }
+          pb[u][t][0] = transpose8x8(pack2<false>(w[0], w[1]));
+          pb[u][t][1] = transpose8x8(pack2<false>(w[2], w[3]));
         }
-        pb[t][0] = transpose8x8(pack2<false>(w[0], w[1]));
-        pb[t][1] = transpose8x8(pack2<false>(w[2], w[3]));
-      }
+    }
+    cp_async_wait<3>();
+    __syncwarp();
+    if (any_here) {
 #pragma unroll
-      for (int k = 0; k < MT; ++k) {
-        const uint32_t sel = (k & 1) ? 0x7362u : 0x5140u;
-        const uint32_t x = __byte_perm(cur.v[0][k >> 1], cur.v[1][k >> 1], sel);
-        const uint32_t y = __byte_perm(cur.v[2][k >> 1], cur.v[3][k >> 1], sel);
-        const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)x), a1 = e4m3x2_to_f16x2((uint16_t)(x >> 16));
-        const uint32_t a2 = e4m3x2_to_f16x2((uint16_t)y), a3 = e4m3x2_to_f16x2((uint16_t)(y >> 16));
+      for (int u = 0; u < SL; ++u) {
+        uint32_t vr[4][D / 32];
+        read_v<D>(vr, stage + (SL + u) * SIDE, g, c);
+        if (left[u] < SLAB) {  // what an earlier owner of the page left, NaN perhaps: 0 * NaN is not 0
 #pragma unroll
-        for (int t = 0; t < NT; ++t) mma_f16(o[k][t], a0, a1, a2, a3, pb[t][0], pb[t][1]);
+          for (int t = 0; t < 4; ++t)
+            if (2 * c + (t & 1) + (t >> 1) * 8 >= left[u]) {
+#pragma unroll
+              for (int k = 0; k < D / 32; ++k) vr[t][k] = 0u;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < MT; ++k) {
+          const uint32_t sel = (k & 1) ? 0x7362u : 0x5140u;
+          const uint32_t x = __byte_perm(vr[0][k >> 1], vr[1][k >> 1], sel);
+          const uint32_t y = __byte_perm(vr[2][k >> 1], vr[3][k >> 1], sel);
+          const uint32_t a0 = e4m3x2_to_f16x2((uint16_t)x), a1 = e4m3x2_to_f16x2((uint16_t)(x >> 16));
+          const uint32_t a2 = e4m3x2_to_f16x2((uint16_t)y), a3 = e4m3x2_to_f16x2((uint16_t)(y >> 16));
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma_f16(o[k][t], a0, a1, a2, a3, pb[u][t][0], pb[u][t][1]);
+        }
       }
     }
-    cur = nxt;
+    __syncwarp();
+    fetch(next, st, 1);
   }
+  cp_async_wait<0>();
 
   // join the warps
 #pragma unroll
@@ -357,7 +435,7 @@ __global__ void __launch_bounds__(THREADS) attn_decode_kernel(const DecodeParams
       }
     }
   if (lane == 0) s_seen[warp] = seen;
-  __syncthreads();  // also: every warp is done with the page entries, whose memory takes O now
+  __syncthreads();  // also: every warp is done with its ring, whose memory takes O now
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -369,8 +447,8 @@ __global__ void __launch_bounds__(THREADS) attn_decode_kernel(const DecodeParams
       const float alpha = ex2(refw[t][j] - top);
       float* dst = so + (warp * ROWS + row) * OSTRIDE;
 #pragma unroll
-      for (int k = 0; k < MT; ++k)  // head-dim indices of lane (g, c), tile k: (D / 8) g + 2k and + 1
-        *reinterpret_cast<float2*>(dst + g * (D / 8) + 2 * k) = make_float2(o[k][t][j] * alpha, o[k][t][j + 2] * alpha);
+      for (int k = 0; k < MT; ++k)
+        *reinterpret_cast<float2*>(dst + v_index<D>(g, k)) = make_float2(o[k][t][j] * alpha, o[k][t][j + 2] * alpha);
     }
   __syncthreads();
   int any = 0;
@@ -405,59 +483,107 @@ __global__ void __launch_bounds__(THREADS) attn_decode_kernel(const DecodeParams
   }
 }
 
-// Joins the chunks of one (sequence, query head) per warp: o = sum_i 2^(lse_i - max) o_i / sum_i 2^(lse_i - max).
+// Joins the chunks of a (sequence, query head): o = sum_i 2^(lse_i - max) o_i / sum_i 2^(lse_i - max).  A CTA
+// each, D / 4 threads over the head dim and the groups of them over the chunks, several loads in flight: one
+// warp that walked 147 chunks took 73 us.
+constexpr int JOIN_MOST = 512;  // weights kept at a time
 template <int D, bool BF16>
 __global__ void __launch_bounds__(THREADS) attn_decode_join_kernel(const DecodeParams p) {
-  constexpr int PER = D / 32;
-  const int lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * WARPS + (threadIdx.x >> 5);
-  if (row >= (long long)p.B * p.Hq) return;
+  constexpr int LANES = D / 4, GROUPS = THREADS / LANES;
+  __shared__ float s_w[JOIN_MOST], s_red[WARPS];
+  __shared__ __align__(16) float s_acc[GROUPS][D];
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // until the chunks' kernel has ended and its writes are seen
+  const int tid = threadIdx.x, lane = tid & 31, d = (tid % LANES) * 4, grp = tid / LANES;
+  const long long row = blockIdx.x;
   const int b = (int)(row / p.Hq), hq = (int)(row % p.Hq);
   const int len = min(max(p.lens[b], 0), p.max_pages * p.page_size);
   const int nslabs = (len + SLAB - 1) / SLAB;
   if (nslabs <= p.chunk) return;  // its only chunk has written the output
   const int n = (nslabs + p.chunk - 1) / p.chunk;
   const float* lse = p.ws_lse + row * p.splits;
-  float top = REF_NONE;
-  for (int i = lane; i < n; i += 32) top = fmaxf(top, lse[i]);
+  const float* src = p.ws_o + row * p.splits * D + d;
+  auto reduce = [&](float x, bool sum) {  // over the CTA, the same bits in every thread
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-  float acc[PER], sum = 0.f;
-  bool any = false;
+    for (int i = 16; i > 0; i >>= 1) {
+      const float y = __shfl_xor_sync(0xffffffffu, x, i);
+      x = sum ? x + y : fmaxf(x, y);
+    }
+    __syncthreads();
+    if (lane == 0) s_red[tid >> 5] = x;
+    __syncthreads();
+    x = s_red[0];
 #pragma unroll
-  for (int j = 0; j < PER; ++j) acc[j] = 0.f;
-  const float* src = p.ws_o + row * p.splits * D + lane * PER;
-  for (int i = 0; i < n; ++i) {
-    const float li = lse[i];
-    if (li == -INFINITY) continue;  // a chunk none of whose pages exists
-    any = true;
-    const float w = ex2(li - top);
-    sum += w;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) acc[j] += w * src[(long long)i * D + j];
+    for (int i = 1; i < WARPS; ++i) x = sum ? x + s_red[i] : fmaxf(x, s_red[i]);
+    return x;
+  };
+  float top = -INFINITY;
+  bool nan = false;  // a chunk of NaN: its row is NaN, which a maximum would pass over
+  for (int i = tid; i < n; i += THREADS) {
+    const float x = lse[i];
+    nan |= x != x;
+    top = fmaxf(top, x);
   }
-  const float f = any ? 1.f / sum : 0.f;
-  uint16_t* dst = p.o + b * p.o_sb + hq * p.o_sh + lane * PER;
+  top = reduce(top, false);
+  nan = __syncthreads_or(nan);
+  const bool any = top != -INFINITY || nan;  // -inf: none of the pages exists
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  for (int i0 = 0; i0 < n; i0 += JOIN_MOST) {
+    const int m = min(JOIN_MOST, n - i0);
+    __syncthreads();
+    for (int i = tid; i < m; i += THREADS) {
+      const float x = lse[i0 + i], w = x == -INFINITY ? 0.f : ex2(x - top);
+      s_w[i] = w;
+      sum += w;
+    }
+    __syncthreads();
+#pragma unroll 8
+    for (int i = grp; i < m; i += GROUPS) {
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(src + (long long)(i0 + i) * D));
+      const float w = s_w[i];
+      acc.x += w * x.x; acc.y += w * x.y; acc.z += w * x.z; acc.w += w * x.w;
+    }
+  }
+  sum = reduce(sum, true);
+  *reinterpret_cast<float4*>(&s_acc[grp][d]) = acc;
+  __syncthreads();
+  if (grp == 0) {
 #pragma unroll
-  for (int j = 0; j < PER; j += 2)
-    *reinterpret_cast<uint32_t*>(dst + j) = pack2<BF16>(acc[j] * f, acc[j + 1] * f);
-  if (lane == 0 && p.m) p.m[row] = any ? top + log2f(sum) : -INFINITY;
+    for (int i = 1; i < GROUPS; ++i) {
+      const float4 x = *reinterpret_cast<const float4*>(&s_acc[i][d]);
+      acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
+    }
+    const float f = any ? 1.f / sum : 0.f;
+    *reinterpret_cast<uint2*>(p.o + b * p.o_sb + hq * p.o_sh + d) =
+        make_uint2(pack2<BF16>(acc.x * f, acc.y * f), pack2<BF16>(acc.z * f, acc.w * f));
+    if (tid == 0 && p.m) p.m[row] = any ? top + log2f(sum) : -INFINITY;
+  }
 }
 
 template <int D, int NT, bool BF16>
 int launch_t(DeviceCtx* ctx, cudaStream_t stream, const DecodeParams& p) {
-  constexpr size_t out_bytes = (size_t)WARPS * 8 * NT * (D + 4) * sizeof(float);
-  constexpr size_t most = MAX_CHUNK_SLABS * sizeof(SlabEntry) > out_bytes ? MAX_CHUNK_SLABS * sizeof(SlabEntry) : out_bytes;
+  static_assert(RING<D> >= 8 * NT * (D + 4) * 4, "the warps' outputs take the rings' place");
+  constexpr size_t most = (size_t)WARPS * RING<D> + MAX_CHUNK_SLABS * sizeof(SlabEntry);
   static std::atomic<bool> attr_done[64];
   if (int rc = ensure_dynamic_smem(attn_decode_kernel<D, NT, BF16>, most, ctx->device, attr_done, "attn decode")) return rc;
-  const size_t table_bytes = (size_t)p.chunk * sizeof(SlabEntry);
-  const size_t smem = table_bytes > out_bytes ? table_bytes : out_bytes;
+  const size_t smem = (size_t)WARPS * RING<D> + (size_t)p.chunk * sizeof(SlabEntry);
   const dim3 grid((unsigned)p.splits, (unsigned)(p.Hkv * p.row_blocks), (unsigned)p.B);
   attn_decode_kernel<D, NT, BF16><<<grid, THREADS, smem, stream>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess && p.splits > 1) {
-    attn_decode_join_kernel<D, BF16><<<(unsigned)(((long long)p.B * p.Hq + WARPS - 1) / WARPS), THREADS, 0, stream>>>(p);
-    e = cudaGetLastError();
+    // launched while the chunks still run (it waits for their end before it reads): its launch latency and
+    // theirs overlap
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)((long long)p.B * p.Hq));
+    cfg.blockDim = dim3(THREADS);
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, attn_decode_join_kernel<D, BF16>, p);
+    if (e == cudaSuccess) e = cudaGetLastError();
   }
   if (e != cudaSuccess) return fail(B200_ERR_CUDA, "attn decode launch: %s", cudaGetErrorString(e));
   return B200_OK;

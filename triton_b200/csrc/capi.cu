@@ -730,7 +730,7 @@ int b200_attention_decode(b200_stream_t stream, const void* q, const void* k_cac
   }
   if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(o) & 15))
     return fail(B200_ERR_UNSUPPORTED, "q and o must be 16-byte aligned");
-  if (batch > 65535 || Hq > 65535) return fail(B200_ERR_UNSUPPORTED, "at most 65535 sequences and heads in a call");
+  if (batch > 65535 || Hq > 32767) return fail(B200_ERR_UNSUPPORTED, "at most 65535 sequences and 32767 heads in a call");
   DeviceCtx* ctx = ready_ctx();
   if (!ctx) return g_err_code;
   if (batch == 0 || Hq == 0) return B200_OK;
