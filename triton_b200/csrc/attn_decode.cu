@@ -31,9 +31,16 @@ namespace {
 
 constexpr int WARPS = 4, THREADS = WARPS * 32;
 constexpr int SLAB = 16;             // tokens of one MMA
-constexpr int MAX_CHUNK_SLABS = 256;  // page-table entries a CTA keeps in shared memory
+constexpr int MAX_CHUNK_SLABS = 256;  // page entries a CTA keeps in shared memory
 constexpr float REF_NONE = -1.7e38f;   // reference point before the first token: finite, below every score
 constexpr float LOG2E = 1.4426950408889634f;
+
+// A warp takes STEP slabs at once (two: independent chains of MMAs) and owns a ring of two such steps in
+// shared memory, K and V refilled as soon as each has been read.
+template <int D> constexpr int STEP = D == 256 ? 1 : 2;
+template <int D> constexpr int RING = 2 * STEP<D> * SLAB * D * 2;
+// CTAs an SM holds (registers and rings)
+template <int D, int NT> constexpr int CTAS = D == 64 ? (NT == 1 ? 6 : 4) : 3;
 
 struct DecodePlan {
   int nt;            // groups of 8 query heads per CTA
@@ -47,15 +54,25 @@ DecodePlan decode_plan(int B, int Hq, int Hkv, int D, int page_size, int max_pag
   const int G = Hq / Hkv;
   p.nt = (G > 8 && D <= 128) ? 2 : 1;
   p.row_blocks = (G + 8 * p.nt - 1) / (8 * p.nt);
-  const long long slabs = (long long)max_pages * (page_size / SLAB);
-  const long long ctas = (long long)B * Hkv * p.row_blocks;
-  const long long want = 148 * 6;
-  long long splits = (want + ctas - 1) / ctas;
-  long long chunk = (slabs + splits - 1) / splits;
-  if (chunk < 8) chunk = 8;
-  if (chunk > MAX_CHUNK_SLABS) chunk = MAX_CHUNK_SLABS;
-  p.chunk = (int)chunk;
-  p.splits = (int)((slabs + chunk - 1) / chunk);
+  const int slabs = max_pages * (page_size / SLAB);
+  const double pairs = (double)B * Hkv * p.row_blocks;
+  const double room = 148.0 * (D == 64 ? (p.nt == 1 ? CTAS<64, 1> : CTAS<64, 2>) : 3);
+  // The chunk that is done first by this estimate, in slab times: a CTA takes its slabs and about 10 more for
+  // its start and its join.  One sequence fills `room` CTAs at once; of several the lengths are not known here,
+  // so half the table is taken as their mean, and the last CTAs to start run half a chunk alone.
+  const int one_wave = pairs < room ? (int)((slabs + (int)(room / pairs) - 1) / (int)(room / pairs)) : MAX_CHUNK_SLABS;
+  const int sizes[] = {8, 16, 24, 32, 48, 64, 96, 128, 192, 256, one_wave};
+  double best = 0;
+  p.chunk = 0;
+  for (int chunk : sizes) {
+    chunk = chunk < 8 ? 8 : chunk > MAX_CHUNK_SLABS ? MAX_CHUNK_SLABS : (chunk + 1) / 2 * 2;
+    const double ctas = pairs * ((slabs + chunk - 1) / chunk);
+    double t;
+    if (B == 1) t = (ctas <= room ? 1.0 : ctas / room + 0.5) * (chunk + 10);
+    else t = ctas * (0.5 * chunk + 10) / room + 0.5 * (chunk + 10);
+    if (p.chunk == 0 || t < best) { best = t; p.chunk = chunk; }
+  }
+  p.splits = (slabs + p.chunk - 1) / p.chunk;
   if (p.splits < 1) p.splits = 1;
   return p;
 }
@@ -77,11 +94,6 @@ struct DecodeParams {
   float* ws_o;    // [B, Hq, splits, D] outputs of the chunks
   float* ws_lse;  // [B, Hq, splits] their base-2 log-sum-exp
 };
-
-// A warp takes STEP slabs at once (two: independent chains of MMAs) and owns a ring of two such steps in
-// shared memory, K and V refilled as soon as each has been read.
-template <int D> constexpr int STEP = D == 256 ? 1 : 2;
-template <int D> constexpr int RING = 2 * STEP<D> * SLAB * D * 2;
 
 struct SlabEntry {
   unsigned slab;  // index of 16-token slabs in the cache (times 16 * D bytes); ~0u: no page
@@ -169,7 +181,7 @@ __device__ __forceinline__ void read_v(uint32_t (&v)[4][D / 32], const uint8_t* 
 }
 
 template <int D, int NT, bool BF16>
-__global__ void __launch_bounds__(THREADS, 3) attn_decode_kernel(const DecodeParams p) {
+__global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const DecodeParams p) {
   constexpr int ROWS = 8 * NT, KSTEPS = D / 16, MT = D / 16;
   constexpr int OSTRIDE = D + 4;  // floats; + 4 spreads the rows over the banks
   constexpr int SL = STEP<D>, SIDE = SLAB * D, STAGE = 2 * SL * SIDE;  // a stage: SL slabs of K, then of V
@@ -184,50 +196,74 @@ __global__ void __launch_bounds__(THREADS, 3) attn_decode_kernel(const DecodePar
   const int split = blockIdx.x, b = blockIdx.z;
   const int h = blockIdx.y / p.row_blocks, rb = blockIdx.y % p.row_blocks;
   const int row0 = rb * ROWS, nrows = min(ROWS, p.G - row0);  // query heads h * G + row0 + [0, nrows)
-  const int len = min(max(p.lens[b], 0), p.max_pages * p.page_size);
+  // Every load of the start that needs no other goes out first: the length, q, the chunk's pages (the table has
+  // room for the chunk whatever the length is); then the bytes are sent for, and the scales after them.
+  const int len_given = __ldg(p.lens + b);
+  const int s0 = split * p.chunk, spp = p.page_size / SLAB, room = p.max_pages * spp;
+  int pages[MAX_CHUNK_SLABS / THREADS];
+#pragma unroll
+  for (int k = 0; k < MAX_CHUNK_SLABS / THREADS; ++k) {
+    const int i = threadIdx.x + k * THREADS;
+    pages[k] = (i < p.chunk && s0 + i < room) ? __ldg(p.table + b * p.table_stride + (s0 + i) / spp) : -1;
+  }
+  // q as the B operand: for k-step s the four head-dim indices of K's word s
+  uint2 raw[NT][KSTEPS];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const uint16_t* qr = p.q + b * p.q_sb + (long long)(h * p.G + row0 + min(t * 8 + g, nrows - 1)) * p.q_sh;
+#pragma unroll
+    for (int s = 0; s < KSTEPS; ++s) raw[t][s] = __ldg(reinterpret_cast<const uint2*>(qr + k_index<D>(c, s)));
+  }
+  const int len = min(max(len_given, 0), p.max_pages * p.page_size);
   const int nslabs = (len + SLAB - 1) / SLAB;
-  const int s0 = split * p.chunk, s1 = min(s0 + p.chunk, nslabs);
+  const int s1 = min(s0 + p.chunk, nslabs), count = s1 - s0;
   if (split > 0 && s0 >= nslabs) return;  // (chunk 0 of an empty sequence writes the zeros)
   const bool whole = nslabs <= p.chunk;
-
-  // this chunk's pages and their scales
-  const int spp = p.page_size / SLAB;
-  for (int i = threadIdx.x; i < s1 - s0; i += THREADS) {
-    const int slab = s0 + i, pg = p.table[b * p.table_stride + slab / spp];
-    SlabEntry e;
-    e.slab = ~0u; e.ks = 0.f; e.ev = 0.f;
-    if (pg >= 0 && pg < p.pages) {  // any other entry names no page: its tokens are left out
-      const unsigned ph = (unsigned)pg * p.Hkv + h;
-      e.slab = ph * spp + slab % spp;
-      e.ks = p.k_scale[ph];
-      e.ev = (float)((int)((__float_as_uint(p.v_scale[ph]) >> 23) & 0xFFu) - 127);
-    }
-    table[i] = e;
+#pragma unroll
+  for (int k = 0; k < MAX_CHUNK_SLABS / THREADS; ++k) {
+    const int i = threadIdx.x + k * THREADS;
+    // any entry that is no page's number names no page: its tokens are left out
+    if (i < count) table[i].slab = (pages[k] >= 0 && pages[k] < p.pages) ? ((unsigned)pages[k] * p.Hkv + h) * spp + (s0 + i) % spp : ~0u;
   }
+  uint8_t* ring = smem + warp * RING<D>;
+  auto fetch = [&](int i, int st, int side) {
+#pragma unroll
+    for (int u = 0; u < SL; ++u)
+      if (i + u < count && table[i + u].slab != ~0u)
+        fetch_slab<D>(smem_u32(ring) + st * STAGE + (side * SL + u) * SIDE, side ? p.v : p.k, table[i + u].slab, lane);
+    cp_async_commit();
+  };
+  __syncthreads();
+#pragma unroll
+  for (int st = 0; st < 2; ++st) {
+    fetch((st * WARPS + warp) * SL, st, 0);
+    fetch((st * WARPS + warp) * SL, st, 1);
+  }
+  for (int i = threadIdx.x; i < count; i += THREADS)
+    if (table[i].slab != ~0u) {
+      const unsigned ph = table[i].slab / spp;
+      table[i].ks = __ldg(p.k_scale + ph);
+      table[i].ev = (float)((int)((__float_as_uint(__ldg(p.v_scale + ph)) >> 23) & 0xFFu) - 127);
+    }
 
-  // q as the B operand: for k-step s the four head-dim indices of K's word s
   uint32_t qf[KSTEPS][NT][2];
   float fac[NT][2];  // per query row 2c, 2c + 1 of each group: score of one unit of the product, log2 units
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
-    const int row = t * 8 + g;
-    const uint16_t* qr = p.q + b * p.q_sb + (long long)(h * p.G + row0 + min(row, nrows - 1)) * p.q_sh;
-    uint2 raw[KSTEPS];
+    if (t * 8 + g >= nrows) {
 #pragma unroll
-    for (int s = 0; s < KSTEPS; ++s) {
-      raw[s] = __ldg(reinterpret_cast<const uint2*>(qr + k_index<D>(c, s)));
-      if (row >= nrows) raw[s] = make_uint2(0, 0);
+      for (int s = 0; s < KSTEPS; ++s) raw[t][s] = make_uint2(0, 0);
     }
     float f = p.sm_scale_log2;
     if constexpr (!BF16) {
 #pragma unroll
-      for (int s = 0; s < KSTEPS; ++s) { qf[s][t][0] = raw[s].x; qf[s][t][1] = raw[s].y; }
+      for (int s = 0; s < KSTEPS; ++s) { qf[s][t][0] = raw[t][s].x; qf[s][t][1] = raw[t][s].y; }
     } else {
       float mx = 0.f;
 #pragma unroll
       for (int s = 0; s < KSTEPS; ++s) {
-        mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(raw[s].x << 16)), fabsf(__uint_as_float(raw[s].x & 0xFFFF0000u))));
-        mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(raw[s].y << 16)), fabsf(__uint_as_float(raw[s].y & 0xFFFF0000u))));
+        mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(raw[t][s].x << 16)), fabsf(__uint_as_float(raw[t][s].x & 0xFFFF0000u))));
+        mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(raw[t][s].y << 16)), fabsf(__uint_as_float(raw[t][s].y & 0xFFFF0000u))));
       }
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
       mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
@@ -238,8 +274,8 @@ __global__ void __launch_bounds__(THREADS, 3) attn_decode_kernel(const DecodePar
       f *= __uint_as_float((uint32_t)(127 - up) << 23);
 #pragma unroll
       for (int s = 0; s < KSTEPS; ++s) {
-        qf[s][t][0] = pack2<false>(__uint_as_float(raw[s].x << 16) * mul, __uint_as_float(raw[s].x & 0xFFFF0000u) * mul);
-        qf[s][t][1] = pack2<false>(__uint_as_float(raw[s].y << 16) * mul, __uint_as_float(raw[s].y & 0xFFFF0000u) * mul);
+        qf[s][t][0] = pack2<false>(__uint_as_float(raw[t][s].x << 16) * mul, __uint_as_float(raw[t][s].x & 0xFFFF0000u) * mul);
+        qf[s][t][1] = pack2<false>(__uint_as_float(raw[t][s].y << 16) * mul, __uint_as_float(raw[t][s].y & 0xFFFF0000u) * mul);
       }
     }
     // row r's factor sits in the lanes 4r .. 4r + 3; this lane's scores are of rows 2c and 2c + 1
@@ -262,20 +298,6 @@ __global__ void __launch_bounds__(THREADS, 3) attn_decode_kernel(const DecodePar
   int seen = 0;
 
   __syncthreads();
-  const int count = s1 - s0;
-  uint8_t* ring = smem + warp * RING<D>;
-  auto fetch = [&](int i, int st, int side) {
-#pragma unroll
-    for (int u = 0; u < SL; ++u)
-      if (i + u < count && table[i + u].slab != ~0u)
-        fetch_slab<D>(smem_u32(ring) + st * STAGE + (side * SL + u) * SIDE, side ? p.v : p.k, table[i + u].slab, lane);
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int st = 0; st < 2; ++st) {
-    fetch((st * WARPS + warp) * SL, st, 0);
-    fetch((st * WARPS + warp) * SL, st, 1);
-  }
   int st = 0;
   for (int i = warp * SL; i < count; i += WARPS * SL, st ^= 1) {
     const uint8_t* stage = ring + st * STAGE;
@@ -286,7 +308,7 @@ __global__ void __launch_bounds__(THREADS, 3) attn_decode_kernel(const DecodePar
 #pragma unroll
     for (int u = 0; u < SL; ++u) {
       SlabEntry e{~0u, 0.f, 0.f};
-      if (u == 0 || i + u < count) e = table[i + u];
+      if ((u == 0 || i + u < count) && table[i + u].slab != ~0u) e = table[i + u];
       ks[u] = e.ks;
       ev[u] = e.ev;
       left[u] = e.slab != ~0u ? len - (s0 + i + u) * SLAB : 0;
@@ -484,9 +506,11 @@ __global__ void __launch_bounds__(THREADS, 3) attn_decode_kernel(const DecodePar
 }
 
 // Joins the chunks of a (sequence, query head): o = sum_i 2^(lse_i - max) o_i / sum_i 2^(lse_i - max).  A CTA
-// each, D / 4 threads over the head dim and the groups of them over the chunks, several loads in flight: one
-// warp that walked 147 chunks took 73 us.
+// each, D / 4 threads over the head dim and the groups of them over the chunks, several loads in flight (one warp
+// that walked 147 chunks took 73 us); a group's first eight are sent for before the weights are known.  It is
+// launched while the chunks still run, so its launch latency is hidden.
 constexpr int JOIN_MOST = 512;  // weights kept at a time
+constexpr int JOIN_AHEAD = 8;
 template <int D, bool BF16>
 __global__ void __launch_bounds__(THREADS) attn_decode_join_kernel(const DecodeParams p) {
   constexpr int LANES = D / 4, GROUPS = THREADS / LANES;
@@ -516,6 +540,12 @@ __global__ void __launch_bounds__(THREADS) attn_decode_join_kernel(const DecodeP
     for (int i = 1; i < WARPS; ++i) x = sum ? x + s_red[i] : fmaxf(x, s_red[i]);
     return x;
   };
+  float4 ahead[JOIN_AHEAD];
+#pragma unroll
+  for (int k = 0; k < JOIN_AHEAD; ++k) {
+    ahead[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (grp + k * GROUPS < n) ahead[k] = __ldcg(reinterpret_cast<const float4*>(src + (long long)(grp + k * GROUPS) * D));
+  }
   float top = -INFINITY;
   bool nan = false;  // a chunk of NaN: its row is NaN, which a maximum would pass over
   for (int i = tid; i < n; i += THREADS) {
@@ -537,8 +567,16 @@ __global__ void __launch_bounds__(THREADS) attn_decode_join_kernel(const DecodeP
       sum += w;
     }
     __syncthreads();
+    int i = grp;
+    if (i0 == 0) {
+#pragma unroll
+      for (int k = 0; k < JOIN_AHEAD; ++k, i += GROUPS) {
+        const float w = i < m ? s_w[i] : 0.f;
+        acc.x += w * ahead[k].x; acc.y += w * ahead[k].y; acc.z += w * ahead[k].z; acc.w += w * ahead[k].w;
+      }
+    }
 #pragma unroll 8
-    for (int i = grp; i < m; i += GROUPS) {
+    for (; i < m; i += GROUPS) {
       const float4 x = __ldcg(reinterpret_cast<const float4*>(src + (long long)(i0 + i) * D));
       const float w = s_w[i];
       acc.x += w * x.x; acc.y += w * x.y; acc.z += w * x.z; acc.w += w * x.w;
@@ -571,13 +609,11 @@ int launch_t(DeviceCtx* ctx, cudaStream_t stream, const DecodeParams& p) {
   attn_decode_kernel<D, NT, BF16><<<grid, THREADS, smem, stream>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess && p.splits > 1) {
-    // launched while the chunks still run (it waits for their end before it reads): its launch latency and
-    // theirs overlap
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)((long long)p.B * p.Hq));
+    cfg.gridDim = dim3((unsigned)(p.B * p.Hq));
     cfg.blockDim = dim3(THREADS);
     cfg.stream = stream;
     cfg.attrs = attr;
