@@ -35,12 +35,16 @@ constexpr int MAX_CHUNK_SLABS = 256;  // page entries a CTA keeps in shared memo
 constexpr float REF_NONE = -1.7e38f;   // reference point before the first token: finite, below every score
 constexpr float LOG2E = 1.4426950408889634f;
 
-// A warp takes STEP slabs at once (two: independent chains of MMAs) and owns a ring of two such steps in
-// shared memory, K and V refilled as soon as each has been read.
+// A warp takes STEP slabs at once (two: independent chains of MMAs) and owns room for one such step in shared
+// memory; K's and V's half are refilled as soon as each has been read, so their bytes have the rest of the
+// step to arrive.  (Room for two steps, hence 12 warps an SM instead of 16, was slower: the loop waits for
+// its own instructions more than for memory.)
 template <int D> constexpr int STEP = D == 256 ? 1 : 2;
-template <int D> constexpr int RING = 2 * STEP<D> * SLAB * D * 2;
-// CTAs an SM holds (registers and rings)
-template <int D, int NT> constexpr int CTAS = D == 64 ? (NT == 1 ? 6 : 4) : 3;
+template <int D> constexpr int ROOM = STEP<D> * SLAB * D * 2;
+// the warps' rooms, in whose place their outputs are joined at the end
+template <int D, int NT> constexpr int AREA = WARPS * (ROOM<D> > 8 * NT * (D + 4) * 4 ? ROOM<D> : 8 * NT * (D + 4) * 4);
+// CTAs an SM holds (registers)
+template <int D, int NT> constexpr int CTAS = D == 64 ? (NT == 1 ? 6 : 4) : D == 128 ? (NT == 1 ? 4 : 3) : 3;
 
 struct DecodePlan {
   int nt;            // groups of 8 query heads per CTA
@@ -56,7 +60,7 @@ DecodePlan decode_plan(int B, int Hq, int Hkv, int D, int page_size, int max_pag
   p.row_blocks = (G + 8 * p.nt - 1) / (8 * p.nt);
   const int slabs = max_pages * (page_size / SLAB);
   const double pairs = (double)B * Hkv * p.row_blocks;
-  const double room = 148.0 * (D == 64 ? (p.nt == 1 ? CTAS<64, 1> : CTAS<64, 2>) : 3);
+  const double room = 148.0 * (D == 64 ? (p.nt == 1 ? CTAS<64, 1> : CTAS<64, 2>) : D == 128 ? (p.nt == 1 ? CTAS<128, 1> : CTAS<128, 2>) : CTAS<256, 1>);
   // The chunk that is done first by this estimate, in slab times: a CTA takes its slabs and about 10 more for
   // its start and its join.  One sequence fills `room` CTAs at once; of several the lengths are not known here,
   // so half the table is taken as their mean, and the last CTAs to start run half a chunk alone.
@@ -95,10 +99,9 @@ struct DecodeParams {
   float* ws_lse;  // [B, Hq, splits] their base-2 log-sum-exp
 };
 
-struct SlabEntry {
-  unsigned slab;  // index of 16-token slabs in the cache (times 16 * D bytes); ~0u: no page
-  float ks;
-  float ev;       // log2 of V's scale
+struct __align__(8) SlabEntry {
+  unsigned slab;    // index of 16-token slabs in the cache (times 16 * D bytes); ~0u: no page
+  unsigned scales;  // exponent fields of K's scale and, 8 bits up, of V's
 };
 
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint16_t x) {
@@ -184,12 +187,12 @@ template <int D, int NT, bool BF16>
 __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const DecodeParams p) {
   constexpr int ROWS = 8 * NT, KSTEPS = D / 16, MT = D / 16;
   constexpr int OSTRIDE = D + 4;  // floats; + 4 spreads the rows over the banks
-  constexpr int SL = STEP<D>, SIDE = SLAB * D, STAGE = 2 * SL * SIDE;  // a stage: SL slabs of K, then of V
-  extern __shared__ __align__(128) uint8_t smem[];  // [WARPS] rings, then the chunk's page entries
-  SlabEntry* table = reinterpret_cast<SlabEntry*>(smem + WARPS * RING<D>);
+  constexpr int SL = STEP<D>, SIDE = SLAB * D;
+  extern __shared__ __align__(128) uint8_t smem[];  // [WARPS] SL slabs of K, then of V; then the chunk's page entries
+  SlabEntry* table = reinterpret_cast<SlabEntry*>(smem + AREA<D, NT>);
   __shared__ float s_refw[WARPS][ROWS], s_refp[WARPS][ROWS], s_l[WARPS][ROWS];
   __shared__ int s_seen[WARPS];
-  float* so = reinterpret_cast<float*>(smem);                                     // [WARPS][ROWS][OSTRIDE], over the rings after the loop
+  float* so = reinterpret_cast<float*>(smem);                                     // [WARPS][ROWS][OSTRIDE], after the loop
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (without a dependent kernel: nothing)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -224,26 +227,24 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
     const int i = threadIdx.x + k * THREADS;
     // any entry that is no page's number names no page: its tokens are left out
     if (i < count) table[i].slab = (pages[k] >= 0 && pages[k] < p.pages) ? ((unsigned)pages[k] * p.Hkv + h) * spp + (s0 + i) % spp : ~0u;
+    else if (i == count) table[i].slab = ~0u;
   }
-  uint8_t* ring = smem + warp * RING<D>;
-  auto fetch = [&](int i, int st, int side) {
+  const uint8_t* room_k = smem + warp * ROOM<D>;
+  const uint8_t* room_v = room_k + SL * SIDE;
+  auto fetch = [&](int i, const uint8_t* dst, const uint8_t* src) {
 #pragma unroll
     for (int u = 0; u < SL; ++u)
-      if (i + u < count && table[i + u].slab != ~0u)
-        fetch_slab<D>(smem_u32(ring) + st * STAGE + (side * SL + u) * SIDE, side ? p.v : p.k, table[i + u].slab, lane);
+      if (i + u < count && table[i + u].slab != ~0u) fetch_slab<D>(smem_u32(dst) + u * SIDE, src, table[i + u].slab, lane);
     cp_async_commit();
   };
   __syncthreads();
-#pragma unroll
-  for (int st = 0; st < 2; ++st) {
-    fetch((st * WARPS + warp) * SL, st, 0);
-    fetch((st * WARPS + warp) * SL, st, 1);
-  }
+  fetch(warp * SL, room_k, p.k);
+  fetch(warp * SL, room_v, p.v);
   for (int i = threadIdx.x; i < count; i += THREADS)
     if (table[i].slab != ~0u) {
       const unsigned ph = table[i].slab / spp;
-      table[i].ks = __ldg(p.k_scale + ph);
-      table[i].ev = (float)((int)((__float_as_uint(__ldg(p.v_scale + ph)) >> 23) & 0xFFu) - 127);
+      const unsigned ks = __float_as_uint(__ldg(p.k_scale + ph)), vs = __float_as_uint(__ldg(p.v_scale + ph));
+      table[i].scales = (ks >> 23 & 0xFFu) | (vs >> 23 & 0xFFu) << 8;
     }
 
   uint32_t qf[KSTEPS][NT][2];
@@ -298,30 +299,26 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
   int seen = 0;
 
   __syncthreads();
-  int st = 0;
-  for (int i = warp * SL; i < count; i += WARPS * SL, st ^= 1) {
-    const uint8_t* stage = ring + st * STAGE;
-    const int next = i + 2 * WARPS * SL;
+  for (int i = warp * SL; i < count; i += WARPS * SL) {
+    const int next = i + WARPS * SL;
     float ks[SL], ev[SL];
     int left[SL];  // tokens of the slab that exist
     bool any_here = false;
 #pragma unroll
     for (int u = 0; u < SL; ++u) {
-      SlabEntry e{~0u, 0.f, 0.f};
-      if ((u == 0 || i + u < count) && table[i + u].slab != ~0u) e = table[i + u];
-      ks[u] = e.ks;
-      ev[u] = e.ev;
+      const SlabEntry e = table[i + u];  // (count is rounded up to SL: the entry behind it says no page)
+      ks[u] = __uint_as_float((e.scales & 0xFFu) << 23);
+      ev[u] = (float)((int)(e.scales >> 8 & 0xFFu) - 127);
       left[u] = e.slab != ~0u ? len - (s0 + i + u) * SLAB : 0;
       any_here |= e.slab != ~0u;
     }
-    // groups were committed in the order K, V of this step, K, V of the next; each wait leaves three
     float s[SL][NT][4];
-    cp_async_wait<3>();
+    cp_async_wait<1>();  // K is here, V may be under way
     __syncwarp();
     if (any_here) {
       uint32_t kr[SL][2][D / 16];
 #pragma unroll
-      for (int u = 0; u < SL; ++u) read_k<D>(kr[u], stage + u * SIDE, g, c);
+      for (int u = 0; u < SL; ++u) read_k<D>(kr[u], room_k + u * SIDE, g, c);
 #pragma unroll
       for (int u = 0; u < SL; ++u)
 #pragma unroll
@@ -340,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
         }
     }
     __syncwarp();
-    fetch(next, st, 0);
+    fetch(next, room_k, p.k);
     uint32_t pb[SL][NT][2];
     if (any_here) {
       seen = 1;
@@ -411,13 +408,13 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
           pb[u][t][1] = transpose8x8(pack2<false>(w[2], w[3]));
         }
     }
-    cp_async_wait<3>();
+    cp_async_wait<1>();  // V is here
     __syncwarp();
     if (any_here) {
 #pragma unroll
       for (int u = 0; u < SL; ++u) {
         uint32_t vr[4][D / 32];
-        read_v<D>(vr, stage + (SL + u) * SIDE, g, c);
+        read_v<D>(vr, room_v + u * SIDE, g, c);
         if (left[u] < SLAB) {  // what an earlier owner of the page left, NaN perhaps: 0 * NaN is not 0
 #pragma unroll
           for (int t = 0; t < 4; ++t)
@@ -439,7 +436,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
       }
     }
     __syncwarp();
-    fetch(next, st, 1);
+    fetch(next, room_v, p.v);
   }
   cp_async_wait<0>();
 
@@ -600,11 +597,10 @@ __global__ void __launch_bounds__(THREADS) attn_decode_join_kernel(const DecodeP
 
 template <int D, int NT, bool BF16>
 int launch_t(DeviceCtx* ctx, cudaStream_t stream, const DecodeParams& p) {
-  static_assert(RING<D> >= 8 * NT * (D + 4) * 4, "the warps' outputs take the rings' place");
-  constexpr size_t most = (size_t)WARPS * RING<D> + MAX_CHUNK_SLABS * sizeof(SlabEntry);
+  constexpr size_t most = (size_t)AREA<D, NT> + (MAX_CHUNK_SLABS + 1) * sizeof(SlabEntry);
   static std::atomic<bool> attr_done[64];
   if (int rc = ensure_dynamic_smem(attn_decode_kernel<D, NT, BF16>, most, ctx->device, attr_done, "attn decode")) return rc;
-  const size_t smem = (size_t)WARPS * RING<D> + (size_t)p.chunk * sizeof(SlabEntry);
+  const size_t smem = (size_t)AREA<D, NT> + (size_t)(p.chunk + 1) * sizeof(SlabEntry);
   const dim3 grid((unsigned)p.splits, (unsigned)(p.Hkv * p.row_blocks), (unsigned)p.B);
   attn_decode_kernel<D, NT, BF16><<<grid, THREADS, smem, stream>>>(p);
   cudaError_t e = cudaGetLastError();
