@@ -32,9 +32,8 @@
 // cu[b + 1].  The tensor maps cover all T rows, a tile starts at the sequence's first row plus a multiple
 // of 128, and what it reads of the next sequence is masked by the length as the ragged end of a dense
 // batch is; the rows of V behind the end are cleared in shared memory before the MMA (they are another
-// sequence's: 0 * inf would reach this one).  The scheduling warp finds the item of a ticket from cu,
-// level by level (the query blocks furthest into their sequences first, heads inside a sequence), and
-// publishes it, so the lengths are never needed on the host.
+// sequence's: 0 * inf would reach this one).  The scheduling warp finds the item of a ticket from cu
+// (PackedWalk) and publishes it, so the lengths are never needed on the host.
 // TMEM columns: S0 [0,128) S1 [128,256) O0 [256,256+D) O1 [384,384+D); P_i = first 64 columns of S_i
 // at head dim 128, and columns [320,384) / [448,512) at head dim 64 (16-bit), where S_i of the next
 // block is then issued before P_i V of this one.  Head dim 256: S [0,128), O [256,512).
@@ -88,6 +87,7 @@ struct FwdParams {
 struct PackedFwdParams : FwdParams {
   const int* cu;    // [batch + 1] offsets into the T rows (N = T, Z = 1, H = Hq)
   int batch, group;  // group: query heads per k/v head
+  int by_level;      // order of the items, see PackedWalk
   int zero_rest;     // rows of o that belong to no sequence: 0 left as they are, 1 set to zero
 };
 
@@ -146,57 +146,70 @@ __device__ __forceinline__ Item decode_item(const FwdParams& p, int w) {
   return it;
 }
 
-// The items of a pack, in the order of their tickets: for every level from the highest down, the
-// sequences with more than `level` query blocks in order, and every head of each.  Warp-collective.
-// Offsets outside [0, T] and negative lengths are cut, so no offset can lead out of the tensors.
+// The items of a pack, in the order of their tickets; tickets only grow, so a walk keeps its place between
+// draws.  Two orders, each made of classes of sequences that the walk counts as it comes to them:
+//   by level   for every query block from the highest down, the sequences that have it, every head of each:
+//              the longest items of the whole pack first, which evens out the end of the launch;
+//   by length  for every number of query blocks from the highest down, the sequences of that length, their
+//              k/v heads in turn, each with its blocks from the last to the first and the heads of its group:
+//              the items that read the same K and V follow one another, which is what counts when the pack's
+//              K and V do not stay in L2.
+// Warp-collective.  Offsets outside [0, T] and negative lengths are cut, so none can lead out of the tensors.
 template <int ROWS>
 struct PackedWalk {
-  int level, base, count, total;  // base: first ticket of the level; count: sequences in it
+  int blocks, base, count, total;  // the class: query blocks, its first ticket, sequences in it
+  bool by_level;
 
   static __device__ __forceinline__ void extent(const PackedFwdParams& p, int b, int& start, int& len) {
     start = min(max(__ldg(p.cu + b), 0), p.N);
     len = max(min(__ldg(p.cu + b + 1), p.N) - start, 0);
   }
-  static __device__ __forceinline__ int blocks(const PackedFwdParams& p, int b) {
+  static __device__ __forceinline__ int seq_blocks(const PackedFwdParams& p, int b) {
     int start, len;
     extent(p, b, start, len);
     return (len + ROWS - 1) / ROWS;
   }
-  __device__ __forceinline__ int count_level(const PackedFwdParams& p) const {
-    int c = 0;
-    for (int b = threadIdx.x & 31; b < p.batch; b += 32) c += blocks(p, b) > level;
-    return (int)__reduce_add_sync(0xffffffffu, (unsigned)c);
+  __device__ __forceinline__ bool in_class(int n) const { return by_level ? n >= blocks : n == blocks; }
+  __device__ __forceinline__ int tickets(const PackedFwdParams& p) const { return count * p.H * (by_level ? 1 : blocks); }
+  // the class of the most blocks below `below`
+  __device__ __forceinline__ void enter(const PackedFwdParams& p, int below) {
+    const int lane = threadIdx.x & 31;
+    int most = 0, c = 0;
+    for (int b = lane; b < p.batch; b += 32) {
+      const int n = seq_blocks(p, b);
+      most = max(most, by_level ? min(n, below - 1) : n < below ? n : 0);
+    }
+    blocks = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);
+    for (int b = lane; b < p.batch; b += 32) c += in_class(seq_blocks(p, b));
+    count = blocks > 0 ? (int)__reduce_add_sync(0xffffffffu, (unsigned)c) : 0;
   }
   __device__ __forceinline__ void init(const PackedFwdParams& p) {
-    int sum = 0, most = 0;
-    for (int b = threadIdx.x & 31; b < p.batch; b += 32) {
-      const int n = blocks(p, b);
-      sum += n;
-      most = max(most, n);
-    }
+    by_level = p.by_level;
+    int sum = 0;
+    for (int b = threadIdx.x & 31; b < p.batch; b += 32) sum += seq_blocks(p, b);
     total = (int)__reduce_add_sync(0xffffffffu, (unsigned)sum) * p.H;
-    level = (int)__reduce_max_sync(0xffffffffu, (unsigned)most) - 1;
     base = 0;
-    count = level >= 0 ? count_level(p) : 0;
+    enter(p, 0x7fffffff);
   }
-  // tickets only grow; w < total
-  __device__ __forceinline__ Item find(const PackedFwdParams& p, int w) {
-    while (w - base >= count * p.H && level > 0) {
-      base += count * p.H;
-      --level;
-      count = count_level(p);
+  __device__ __forceinline__ Item find(const PackedFwdParams& p, int w) {  // w < total
+    while (blocks > 0 && w - base >= tickets(p)) {
+      base += tickets(p);
+      enter(p, blocks);
     }
-    const int nth = (w - base) / p.H, lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, per_seq = p.H * (by_level ? 1 : blocks), per_kv = p.group * (by_level ? 1 : blocks);
+    const int nth = (w - base) / per_seq;
+    int r = (w - base) - nth * per_seq;
     Item it;
-    it.h = (w - base) - nth * p.H;
-    it.kh = it.h / p.group;
-    it.qb = level;
+    it.kh = r / per_kv;
+    r -= it.kh * per_kv;
+    it.qb = blocks - 1 - r / p.group;  // (by level r < group)
+    it.h = it.kh * p.group + r % p.group;
     it.z = it.zh = 0;
     it.row0 = it.N = 0;
     int before = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 32) {
       const int b = b0 + lane;
-      const unsigned in = __ballot_sync(0xffffffffu, b < p.batch && blocks(p, b) > level);
+      const unsigned in = __ballot_sync(0xffffffffu, b < p.batch && in_class(seq_blocks(p, b)));
       const int here = __popc(in);
       if (nth < before + here) {
         const bool me = ((in >> lane) & 1u) && __popc(in & ((1u << lane) - 1u)) == nth - before;
