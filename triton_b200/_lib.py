@@ -74,6 +74,27 @@ def lib():
     return _lib
 
 
+_binding = None
+
+
+def binding():
+    """The compiled binding of the serving calls, bound to the library that lib() has loaded."""
+    global _binding
+    if _binding is None:
+        try:
+            import torch  # noqa: F401  (its libraries, which the binding is linked against)
+            from . import _binding as b
+        except ImportError as e:
+            raise RuntimeError(f"triton_b200/_binding.so cannot be loaded ({e}): build it with `python -m triton_b200.build`; "
+                               "there is no fallback implementation") from e
+        L = lib()
+        b.bind({n: ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in
+                ("b200_attention_varlen_fwd", "b200_kv_append", "b200_attention_decode", "b200_attention_decode_workspace",
+                 "b200_last_error")})
+        _binding = b
+    return _binding
+
+
 def last_error():
     return lib().b200_last_error().decode()
 
@@ -85,10 +106,6 @@ def check(code, what):
 
 def strides4(t):
     return _s4(*t.stride())
-
-
-def strides3(t):
-    return _s3(*t.stride())
 
 
 def status(clear=True):

@@ -6,6 +6,8 @@ Each .cu under csrc/ is compiled to an object next to the library (stale objects
 rebuilt when the source or a header is newer) and linked with the static CUDA runtime;
 the driver API is reached through cudaGetDriverEntryPoint, so the library loads on a
 machine without a GPU driver (it then reports B200_ERR_DEVICE from every compute call).
+csrc/binding.cpp becomes `triton_b200/_binding.so`, the Python binding of the serving calls: host code
+against torch's headers, which calls the library through the addresses that _lib.py hands it.
 """
 import argparse
 import os
@@ -19,6 +21,7 @@ CSRC = os.path.join(PKG, "csrc")
 ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "libtriton_b200.so")
 OBJ = os.path.join(PKG, "csrc", "_obj")
+BINDING = os.path.join(PKG, "_binding.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -39,6 +42,29 @@ def _newest_header():
         if f.endswith((".h", ".cuh")):
             t = max(t, os.path.getmtime(os.path.join(CSRC, f)))
     return t
+
+
+def build_binding(force=False, verbose=False):
+    src = os.path.join(CSRC, "binding.cpp")
+    newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(ROOT, "include", "triton_b200.h")))
+    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= newest:
+        return BINDING
+    import sysconfig
+    import torch
+    home = os.path.dirname(os.path.abspath(torch.__file__))
+    inc = os.path.join(home, "include")
+    cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           "-isystem", inc, "-isystem", os.path.join(inc, "torch", "csrc", "api", "include"),
+           "-isystem", os.path.join(cuda, "include"), "-isystem", sysconfig.get_paths()["include"], src, "-o", BINDING,
+           "-L" + os.path.join(home, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if verbose or r.returncode != 0:
+        sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
+    if r.returncode != 0:
+        raise RuntimeError("the compiler failed for binding.cpp")
+    return BINDING
 
 
 def build(force=False, verbose=False, trace=False):
@@ -65,6 +91,10 @@ def build(force=False, verbose=False, trace=False):
         r = subprocess.run(cmd, capture_output=True, text=True)
         return cmd, r
 
+    binding = None
+    pool = ThreadPoolExecutor(max_workers=1)
+    if not trace:
+        binding = pool.submit(build_binding, force, verbose)  # beside nvcc
     if jobs:
         with ThreadPoolExecutor(max_workers=min(8, len(jobs))) as ex:
             for cmd, r in ex.map(run, jobs):
@@ -79,6 +109,8 @@ def build(force=False, verbose=False, trace=False):
         if r.returncode != 0:
             sys.stderr.write(r.stdout + r.stderr)
             raise RuntimeError("link failed")
+    if binding is not None:
+        binding.result()
     return LIB
 
 

@@ -15,20 +15,9 @@ every call can be captured into a CUDA graph (whose replays see the tensors' cur
 import torch
 
 from . import _lib
-from .ops import _DT, _on_device, _require_cuda, _stream
 
 _HEAD_DIMS = (64, 128, 256)
 _PAGE_SIZES = (16, 32, 64, 128)
-
-
-def _no_grad(what, *ts):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
-        raise RuntimeError(f"{what} has no backward: call it under torch.no_grad(), or attention() for training")
-
-
-def _check_ints(name, t, shape):
-    assert t.dtype == torch.int32 and tuple(t.shape) == shape, f"{name} must be an int32 tensor of shape {shape}"
-    assert t.is_contiguous(), f"{name} must be contiguous"
 
 
 def attention_varlen(q, k, v, cu_seqlens, causal, sm_scale, *, out=None, return_stats=False):
@@ -42,51 +31,15 @@ def attention_varlen(q, k, v, cu_seqlens, causal, sm_scale, *, out=None, return_
     Rows of T that belong to no sequence (padding behind the last one) come back as zeros (-inf in M); with
     `out=` they stay as they were.
     """
-    assert q.dim() == 3 and k.dim() == 3 and v.shape == k.shape, "q [T, Hq, D], k and v [T, Hkv, D]"
-    T, Hq, D = q.shape
-    Hkv = k.shape[1]
-    assert k.shape[0] == T and k.shape[2] == D, "q, k and v must have the same rows and head dim"
-    assert Hkv > 0 and Hq % Hkv == 0, "the query heads must be a multiple of the k/v heads"
-    assert D in (16, 32) + _HEAD_DIMS, f"unsupported head dim {D}"
-    assert q.dtype in (torch.float16, torch.bfloat16) and k.dtype == q.dtype and v.dtype == q.dtype, "fp16 or bf16, one type"
-    assert cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1, "cu_seqlens holds one offset more than there are sequences"
-    _check_ints("cu_seqlens", cu_seqlens, (cu_seqlens.numel(),))
-    _no_grad("attention_varlen", q, k, v)
-    dev = _require_cuda(q, k, v, cu_seqlens)
-    if out is not None:
-        assert out.shape == q.shape and out.dtype == q.dtype and out.device == dev, "out= must look like q"
-    if D in (16, 32):  # as in attention_forward: zero-padded to the kernels' head dim 64
+    if q.dim() == 3 and q.shape[2] in (16, 32):  # as in attention_forward: zero-padded to the kernels' head dim 64
+        D = q.shape[2]
+        assert k.shape[-1] == v.shape[-1] == D, "q, k and v must have the same head dim"
         wide = lambda t: torch.nn.functional.pad(t, (0, 64 - D))
         res = attention_varlen(wide(q), wide(k), wide(v), cu_seqlens, causal, sm_scale,
                                out=None if out is None else wide(out), return_stats=True)
         o = res[0][..., :D].contiguous() if out is None else out.copy_(res[0][..., :D])
         return (o, res[1]) if return_stats else o
-    with _on_device(dev):
-        o = torch.empty((T, Hq, D), device=dev, dtype=q.dtype) if out is None else out
-        M = torch.empty((Hq, T), device=dev, dtype=torch.float32) if return_stats else None
-        code = _lib.lib().b200_attention_varlen_fwd(
-            _stream(q), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), M.data_ptr() if return_stats else None,
-            cu_seqlens.data_ptr(), cu_seqlens.numel() - 1, T, Hq, Hkv, D, _lib.strides3(q), _lib.strides3(k),
-            _lib.strides3(v), _lib.strides3(o), float(sm_scale), 1 if causal else 0, _DT[q.dtype], 1 if out is None else 0)
-        _lib.check(code, "attention_varlen")
-    return (o, M) if return_stats else o
-
-
-def _check_cache(k_cache, v_cache, k_scale, v_scale, page_table, seq_lens):
-    """The cache's tensors belong together; returns (pages, Hkv, page size, head dim)."""
-    assert k_cache.dim() == 4 and v_cache.shape == k_cache.shape, "caches are [pages, Hkv, page size, D]"
-    assert k_cache.dtype == v_cache.dtype == torch.float8_e4m3fn, "caches hold float8_e4m3fn values"
-    assert k_cache.is_contiguous() and v_cache.is_contiguous(), "caches must be contiguous"
-    pages, heads, page, D = k_cache.shape
-    assert page in _PAGE_SIZES, f"pages hold 16, 32, 64 or 128 tokens, not {page}"
-    assert D in _HEAD_DIMS, f"a cache has head dim 64, 128 or 256, not {D}"
-    for name, s in (("k_scale", k_scale), ("v_scale", v_scale)):
-        assert s.dtype == torch.float32 and tuple(s.shape) == (pages, heads) and s.is_contiguous(), \
-            f"{name} must be a contiguous fp32 tensor [pages, Hkv]"
-    assert page_table.dim() == 2 and page_table.dtype == torch.int32 and (page_table.stride(1) == 1 or page_table.shape[1] <= 1), \
-        "page_table must be an int32 tensor [batch, pages of the longest sequence] with contiguous rows"
-    _check_ints("seq_lens", seq_lens, (page_table.shape[0],))
-    return pages, heads, page, D
+    return (_lib._binding or _lib.binding()).attention_varlen(q, k, v, cu_seqlens, causal, sm_scale, out, return_stats)
 
 
 def kv_cache_append(k_cache, v_cache, k_scale, v_scale, k, v, page_table, seq_lens, cu_seqlens=None):
@@ -102,25 +55,7 @@ def kv_cache_append(k_cache, v_cache, k_scale, v_scale, k, v, page_table, seq_le
     When later rows need a larger scale the page's earlier rows are rounded to it.  The stored bytes depend on
     nothing else.  Two sequences of one call may not write to the same page.
     """
-    pages, heads, page, D = _check_cache(k_cache, v_cache, k_scale, v_scale, page_table, seq_lens)
-    batch = page_table.shape[0]
-    assert k.dim() == 3 and tuple(k.shape[1:]) == (heads, D) and v.shape == k.shape, "k and v must be [T, Hkv, D] of the cache's heads"
-    assert k.dtype in (torch.float16, torch.bfloat16) and v.dtype == k.dtype, "fp16 or bf16, one type"
-    tensors = (k_cache, v_cache, k_scale, v_scale, k, v, page_table, seq_lens)
-    if cu_seqlens is None:
-        assert k.shape[0] == batch, "without cu_seqlens every sequence has one new row"
-    else:
-        _check_ints("cu_seqlens", cu_seqlens, (batch + 1,))
-        tensors += (cu_seqlens,)
-    _no_grad("kv_cache_append", k, v)
-    dev = _require_cuda(*tensors)
-    with _on_device(dev):
-        code = _lib.lib().b200_kv_append(
-            _stream(k), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, page,
-            page_table.data_ptr(), page_table.stride(0), page_table.shape[1], seq_lens.data_ptr(), k.data_ptr(), v.data_ptr(),
-            None if cu_seqlens is None else cu_seqlens.data_ptr(), batch, k.shape[0], heads, D, _lib.strides3(k),
-            _lib.strides3(v), _DT[k.dtype])
-        _lib.check(code, "kv_cache_append")
+    (_lib._binding or _lib.binding()).kv_cache_append(k_cache, v_cache, k_scale, v_scale, k, v, page_table, seq_lens, cu_seqlens)
 
 
 def attention_decode(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, sm_scale, *, out=None, return_stats=False):
@@ -128,29 +63,8 @@ def attention_decode(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens
     of the cache's heads, over the first seq_lens[b] tokens (the new one among them, once it is appended).  Tokens
     of a page that the table does not name are left out; a sequence without tokens gives zeros.  Returns O like
     q, with return_stats=True (O, M): M [batch, Hq] is the base-2 log-sum-exp (-inf without tokens)."""
-    pages, heads, page, D = _check_cache(k_cache, v_cache, k_scale, v_scale, page_table, seq_lens)
-    batch = page_table.shape[0]
-    assert q.dim() == 3 and q.shape[0] == batch and q.shape[2] == D, "q must be [batch, Hq, D] of the cache's head dim"
-    Hq = q.shape[1]
-    assert heads > 0 and Hq % heads == 0, "the query heads must be a multiple of the cache's heads"
-    assert q.dtype in (torch.float16, torch.bfloat16), "fp16 or bf16"
-    _no_grad("attention_decode", q)
-    dev = _require_cuda(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens)
-    if out is not None:
-        assert out.shape == q.shape and out.dtype == q.dtype and out.device == dev, "out= must look like q"
-    with _on_device(dev):
-        L = _lib.lib()
-        o = torch.empty((batch, Hq, D), device=dev, dtype=q.dtype) if out is None else out
-        M = torch.empty((batch, Hq), device=dev, dtype=torch.float32) if return_stats else None
-        ws_bytes = L.b200_attention_decode_workspace(batch, Hq, heads, D, page, page_table.shape[1])
-        ws = torch.empty(ws_bytes // 4, device=dev, dtype=torch.float32) if ws_bytes else None
-        code = L.b200_attention_decode(
-            _stream(q), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages,
-            page, page_table.data_ptr(), page_table.stride(0), page_table.shape[1], seq_lens.data_ptr(), o.data_ptr(),
-            M.data_ptr() if return_stats else None, batch, Hq, heads, D, _lib.strides3(q), _lib.strides3(o),
-            float(sm_scale), _DT[q.dtype], None if ws is None else ws.data_ptr())
-        _lib.check(code, "attention_decode")
-    return (o, M) if return_stats else o
+    return (_lib._binding or _lib.binding()).attention_decode(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, sm_scale,
+                                                              out, return_stats)
 
 
 class PagedKVCache:
