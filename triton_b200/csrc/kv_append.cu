@@ -192,19 +192,20 @@ __global__ void __launch_bounds__(PAGE_THREADS) kv_append_page_kernel(const KvAp
   if (page < 0 || page >= a.c.pages) return;  // names no page: its rows are not written
   const int lo = max(start - p * P, 0), hi = min(len - p * P, P);
   const long long t = t0 + (p * P + lo - start);
-  const int per_row = D / 8, items = (hi - lo) * per_row;  // 16 bytes each
+  const int shift = 31 - __clz(D / 8), items = (hi - lo) << shift;  // of 16 bytes, D / 8 (a power of two) a row
+  const int row = tid >> shift, col = (tid & (D / 8 - 1)) * 8;      // of this thread's first
   const int first = blockIdx.y * pairs, last = min(first + pairs, 2 * a.c.Hkv);
 
   auto load = [&](uint4 (&x)[ITEMS], float& held, int pair) {
     const int side = pair & 1, h = pair >> 1;
     const long long st = side ? a.v_st : a.k_st;
     const uint16_t* src = (side ? reinterpret_cast<const uint16_t*>(a.v) + h * a.v_sh
-                                : reinterpret_cast<const uint16_t*>(a.k) + h * a.k_sh) + t * st;
+                                : reinterpret_cast<const uint16_t*>(a.k) + h * a.k_sh) + (t + row) * st + col;
+    const long long step = (PAGE_THREADS >> shift) * st;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-      const int w = i * PAGE_THREADS + tid;
       x[i] = make_uint4(0, 0, 0, 0);
-      if (w < items) x[i] = __ldg(reinterpret_cast<const uint4*>(src + (w / per_row) * st) + w % per_row);
+      if (i * PAGE_THREADS + tid < items) x[i] = __ldg(reinterpret_cast<const uint4*>(src + i * step));
     }
     held = (side ? a.c.v_scale : a.c.k_scale)[(long long)page * a.c.Hkv + h];
   };
