@@ -86,7 +86,7 @@ struct DecodeParams {
   const float *k_scale, *v_scale;
   const int* table;
   long long table_stride;
-  int pages, page_size, max_pages, Hkv;
+  int pages, page_size, page_shift, max_pages, Hkv;  // page_size: 16 << page_shift
   const uint16_t* q;
   uint16_t* o;
   float* m;
@@ -202,12 +202,12 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
   // Every load of the start that needs no other goes out first: the length, q, the chunk's pages (the table has
   // room for the chunk whatever the length is); then the bytes are sent for, and the scales after them.
   const int len_given = __ldg(p.lens + b);
-  const int s0 = split * p.chunk, spp = p.page_size / SLAB, room = p.max_pages * spp;
+  const int s0 = split * p.chunk, sh = p.page_shift, room = p.max_pages << sh;  // 2^sh slabs a page
   int pages[MAX_CHUNK_SLABS / THREADS];
 #pragma unroll
   for (int k = 0; k < MAX_CHUNK_SLABS / THREADS; ++k) {
     const int i = threadIdx.x + k * THREADS;
-    pages[k] = (i < p.chunk && s0 + i < room) ? __ldg(p.table + b * p.table_stride + (s0 + i) / spp) : -1;
+    pages[k] = (i < p.chunk && s0 + i < room) ? __ldg(p.table + b * p.table_stride + ((s0 + i) >> sh)) : -1;
   }
   // q as the B operand: for k-step s the four head-dim indices of K's word s
   uint2 raw[NT][KSTEPS];
@@ -226,8 +226,8 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
   for (int k = 0; k < MAX_CHUNK_SLABS / THREADS; ++k) {
     const int i = threadIdx.x + k * THREADS;
     // any entry that is no page's number names no page: its tokens are left out
-    if (i < count) table[i].slab = (pages[k] >= 0 && pages[k] < p.pages) ? ((unsigned)pages[k] * p.Hkv + h) * spp + (s0 + i) % spp : ~0u;
-    else if (i == count) table[i].slab = ~0u;
+    if (i < count) table[i].slab = (pages[k] >= 0 && pages[k] < p.pages) ? (((unsigned)pages[k] * p.Hkv + h) << sh) + ((s0 + i) & ((1 << sh) - 1)) : ~0u;
+    else if (i < (count + SL - 1) / SL * SL) table[i].slab = ~0u;  // a step may reach past the last slab
   }
   const uint8_t* room_k = smem + warp * ROOM<D>;
   const uint8_t* room_v = room_k + SL * SIDE;
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
   fetch(warp * SL, room_v, p.v);
   for (int i = threadIdx.x; i < count; i += THREADS)
     if (table[i].slab != ~0u) {
-      const unsigned ph = table[i].slab / spp;
+      const unsigned ph = table[i].slab >> sh;
       const unsigned ks = __float_as_uint(__ldg(p.k_scale + ph)), vs = __float_as_uint(__ldg(p.v_scale + ph));
       table[i].scales = (ks >> 23 & 0xFFu) | (vs >> 23 & 0xFFu) << 8;
     }
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
     bool any_here = false;
 #pragma unroll
     for (int u = 0; u < SL; ++u) {
-      const SlabEntry e = table[i + u];  // (count is rounded up to SL: the entry behind it says no page)
+      const SlabEntry e = table[i + u];
       ks[u] = __uint_as_float((e.scales & 0xFFu) << 23);
       ev[u] = (float)((int)(e.scales >> 8 & 0xFFu) - 127);
       left[u] = e.slab != ~0u ? len - (s0 + i + u) * SLAB : 0;
@@ -347,7 +347,8 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[u][t][j] = (s[u][t][j] * fac[t][j & 1]) * ks[u];
+          for (int j = 0; j < 4; j += 2)  // two query rows at a time
+            upk2(mul2(mul2(pk2(s[u][t][j], s[u][t][j + 1]), pk2(fac[t][0], fac[t][1])), pk2(ks[u], ks[u])), s[u][t][j], s[u][t][j + 1]);
         if (left[u] < SLAB) {
 #pragma unroll
           for (int t = 0; t < NT; ++t)
@@ -398,12 +399,19 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
       for (int u = 0; u < SL; ++u)
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          float w[4];
+          float w[4], q[4];
+          const uint64_t ew = pk2(ev[u] - refw[t][0], ev[u] - refw[t][1]), ep = pk2(-refp[t][0], -refp[t][1]);
+          uint64_t sum = pk2(l[t][0], l[t][1]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            w[j] = ex2(s[u][t][j] + (ev[u] - refw[t][j & 1]));
-            l[t][j & 1] += ex2(s[u][t][j] - refp[t][j & 1]);
+          for (int j = 0; j < 4; j += 2) {
+            const uint64_t x = pk2(s[u][t][j], s[u][t][j + 1]);
+            upk2(add2(x, ew), w[j], w[j + 1]);
+            upk2(add2(x, ep), q[j], q[j + 1]);
+            w[j] = ex2(w[j]);
+            w[j + 1] = ex2(w[j + 1]);
+            sum = add2(sum, pk2(ex2(q[j]), ex2(q[j + 1])));
           }
+          upk2(sum, l[t][0], l[t][1]);
           pb[u][t][0] = transpose8x8(pack2<false>(w[0], w[1]));
           pb[u][t][1] = transpose8x8(pack2<false>(w[2], w[3]));
         }
@@ -640,7 +648,7 @@ int launch_attn_decode(DeviceCtx* ctx, cudaStream_t stream, const AttnDecodeArgs
   DecodeParams p{};
   p.k = a.c.k; p.v = a.c.v; p.k_scale = a.c.k_scale; p.v_scale = a.c.v_scale;
   p.table = a.c.table; p.table_stride = a.c.table_stride;
-  p.pages = a.c.pages; p.page_size = a.c.page_size; p.max_pages = a.c.max_pages; p.Hkv = a.c.Hkv;
+  p.pages = a.c.pages; p.page_size = a.c.page_size; p.page_shift = a.c.page_size == 16 ? 0 : a.c.page_size == 32 ? 1 : a.c.page_size == 64 ? 2 : 3; p.max_pages = a.c.max_pages; p.Hkv = a.c.Hkv;
   p.q = static_cast<const uint16_t*>(a.q); p.o = static_cast<uint16_t*>(a.o); p.m = a.m;
   p.q_sb = a.q_sb; p.q_sh = a.q_sh; p.o_sb = a.o_sb; p.o_sh = a.o_sh;
   p.lens = a.lens; p.B = a.B; p.Hq = a.Hq; p.G = a.Hq / a.c.Hkv; p.row_blocks = pl.row_blocks;
