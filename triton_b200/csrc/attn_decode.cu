@@ -51,6 +51,7 @@ struct DecodePlan {
   int row_blocks;    // CTAs over the query heads of one k/v head
   int chunk;         // slabs per CTA
   int splits;        // chunks of the longest sequence the page table has room for
+  bool cluster;      // a sequence's chunks are one cluster and join in shared memory
 };
 
 DecodePlan decode_plan(int B, int Hq, int Hkv, int D, int page_size, int max_pages) {
@@ -78,6 +79,21 @@ DecodePlan decode_plan(int B, int Hq, int Hkv, int D, int page_size, int max_pag
   }
   p.splits = (slabs + p.chunk - 1) / p.chunk;
   if (p.splits < 1) p.splits = 1;
+  // Few CTAs: up to eight chunks as a cluster, without workspace and second kernel.  Chunks twice as long cost the
+  // GPU about what the second kernel does (1900 tokens of 32/8 heads: 8 slabs and a join 6.3 us, 16 in a cluster of
+  // eight 6.2 us) and the host a launch and an allocation less (9.3 against 5.9 us).  Only where all CTAs
+  // are resident at once: those without tokens wait for their cluster's others.
+  p.cluster = false;
+  if (p.splits > 1) {
+    int size = 2;
+    while (size < 8 && (slabs + size - 1) / size > 8) size *= 2;
+    const int chunk = ((slabs + size - 1) / size + 1) / 2 * 2;
+    if (pairs * size <= room && chunk <= p.chunk + 16 && chunk <= MAX_CHUNK_SLABS) {
+      p.cluster = true;
+      p.chunk = chunk;
+      p.splits = size;
+    }
+  }
   return p;
 }
 
@@ -183,7 +199,24 @@ __device__ __forceinline__ void read_v(uint32_t (&v)[4][D / 32], const uint8_t* 
   }
 }
 
-template <int D, int NT, bool BF16>
+// shared memory of the cluster's CTA `rank`, at the place of this CTA's `p`
+__device__ __forceinline__ uint32_t in_cluster(const float* p, int rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float4 ld_cluster4(const float* p, int rank) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(in_cluster(p, rank)) : "memory");
+  return x;
+}
+__device__ __forceinline__ float ld_cluster(const float* p, int rank) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(in_cluster(p, rank)) : "memory");
+  return x;
+}
+
+template <int D, int NT, bool BF16, bool CLUSTER>
 __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const DecodeParams p) {
   constexpr int ROWS = 8 * NT, KSTEPS = D / 16, MT = D / 16;
   constexpr int OSTRIDE = D + 4;  // floats; + 4 spreads the rows over the banks
@@ -192,9 +225,10 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
   SlabEntry* table = reinterpret_cast<SlabEntry*>(smem + AREA<D, NT>);
   __shared__ float s_refw[WARPS][ROWS], s_refp[WARPS][ROWS], s_l[WARPS][ROWS];
   __shared__ int s_seen[WARPS];
+  __shared__ float s_lse[ROWS];
   float* so = reinterpret_cast<float*>(smem);                                     // [WARPS][ROWS][OSTRIDE], after the loop
 
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (without a dependent kernel: nothing)
+  if constexpr (!CLUSTER) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (none waiting: nothing)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
   const int split = blockIdx.x, b = blockIdx.z;
   const int h = blockIdx.y / p.row_blocks, rb = blockIdx.y % p.row_blocks;
@@ -220,8 +254,12 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
   const int len = min(max(len_given, 0), p.max_pages * p.page_size);
   const int nslabs = (len + SLAB - 1) / SLAB;
   const int s1 = min(s0 + p.chunk, nslabs), count = s1 - s0;
-  if (split > 0 && s0 >= nslabs) return;  // (chunk 0 of an empty sequence writes the zeros)
   const bool whole = nslabs <= p.chunk;
+  if (split > 0 && s0 >= nslabs) {  // (chunk 0 of an empty sequence writes the zeros)
+    if constexpr (CLUSTER)
+      if (!whole) { cluster_sync(); cluster_sync(); }
+    return;
+  }
 #pragma unroll
   for (int k = 0; k < MAX_CHUNK_SLABS / THREADS; ++k) {
     const int i = threadIdx.x + k * THREADS;
@@ -502,11 +540,56 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
       uint16_t* dst = p.o + b * p.o_sb + hq * p.o_sh + d;
       *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<BF16>(x.x, x.y), pack2<BF16>(x.z, x.w));
       if (d == 0 && p.m) p.m[(long long)b * p.Hq + hq] = lse;
+    } else if constexpr (CLUSTER) {
+      *reinterpret_cast<float4*>(so + row * OSTRIDE + d) = x;  // (only this thread has read the place)
+      if (d == 0) s_lse[row] = lse;
     } else {
       const long long at = ((long long)b * p.Hq + hq) * p.splits + split;
       *reinterpret_cast<float4*>(p.ws_o + at * D + d) = x;
       if (d == 0) p.ws_lse[at] = lse;
     }
+  }
+  if constexpr (CLUSTER) {
+    if (whole) return;  // the same for every CTA of the cluster: none waits
+    __syncwarp();
+    cluster_sync();  // every chunk's output and log-sum-exp are in its CTA's shared memory
+    const int parts = (nslabs + p.chunk - 1) / p.chunk;
+    for (int i = split * THREADS + threadIdx.x; i < nrows * (D / 4); i += parts * THREADS) {
+      const int row = i / (D / 4), d = i % (D / 4) * 4;
+      float4 part[8];
+      float lse[8], top = -INFINITY;
+      bool nan = false;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        part[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        lse[k] = -INFINITY;
+        if (k < parts) {
+          part[k] = ld_cluster4(so + row * OSTRIDE + d, k);
+          lse[k] = ld_cluster(s_lse + row, k);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        nan |= lse[k] != lse[k];
+        top = fmaxf(top, lse[k]);
+      }
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float w = lse[k] == -INFINITY ? 0.f : ex2(lse[k] - top);  // (-inf: none of its pages exists)
+        sum += w;
+        x.x += w * part[k].x; x.y += w * part[k].y; x.z += w * part[k].z; x.w += w * part[k].w;
+      }
+      const bool tokens = top != -INFINITY || nan;
+      const float f = tokens ? 1.f / sum : 0.f;
+      const long long hq = h * p.G + row0 + row;
+      *reinterpret_cast<uint2*>(p.o + b * p.o_sb + hq * p.o_sh + d) =
+          make_uint2(pack2<BF16>(x.x * f, x.y * f), pack2<BF16>(x.z * f, x.w * f));
+      if (d == 0 && p.m) p.m[(long long)b * p.Hq + hq] = tokens ? top + log2f(sum) : -INFINITY;
+    }
+    __syncwarp();
+    cluster_sync();  // nobody reads this CTA's shared memory any more
   }
 }
 
@@ -516,9 +599,9 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
 // launched while the chunks still run, so its launch latency is hidden.
 constexpr int JOIN_MOST = 512;  // weights kept at a time
 constexpr int JOIN_AHEAD = 8;
-template <int D, bool BF16>
+template <int D, bool BF16, int THREADS>
 __global__ void __launch_bounds__(THREADS) attn_decode_join_kernel(const DecodeParams p) {
-  constexpr int LANES = D / 4, GROUPS = THREADS / LANES;
+  constexpr int LANES = D / 4, GROUPS = THREADS / LANES, WARPS = THREADS / 32;
   __shared__ float s_w[JOIN_MOST], s_red[WARPS];
   __shared__ __align__(16) float s_acc[GROUPS][D];
   asm volatile("griddepcontrol.wait;" ::: "memory");  // until the chunks' kernel has ended and its writes are seen
@@ -603,44 +686,62 @@ __global__ void __launch_bounds__(THREADS) attn_decode_join_kernel(const DecodeP
   }
 }
 
-template <int D, int NT, bool BF16>
+template <int D, int NT, bool BF16, bool CLUSTER>
 int launch_t(DeviceCtx* ctx, cudaStream_t stream, const DecodeParams& p) {
-  constexpr size_t most = (size_t)AREA<D, NT> + (MAX_CHUNK_SLABS + 1) * sizeof(SlabEntry);
+  constexpr size_t most = (size_t)AREA<D, NT> + (MAX_CHUNK_SLABS + STEP<D>) * sizeof(SlabEntry);
   static std::atomic<bool> attr_done[64];
-  if (int rc = ensure_dynamic_smem(attn_decode_kernel<D, NT, BF16>, most, ctx->device, attr_done, "attn decode")) return rc;
-  const size_t smem = (size_t)AREA<D, NT> + (size_t)(p.chunk + 1) * sizeof(SlabEntry);
-  const dim3 grid((unsigned)p.splits, (unsigned)(p.Hkv * p.row_blocks), (unsigned)p.B);
-  attn_decode_kernel<D, NT, BF16><<<grid, THREADS, smem, stream>>>(p);
-  cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess && p.splits > 1) {
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr[1];
+  if (int rc = ensure_dynamic_smem(attn_decode_kernel<D, NT, BF16, CLUSTER>, most, ctx->device, attr_done, "attn decode")) return rc;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3((unsigned)p.splits, (unsigned)(p.Hkv * p.row_blocks), (unsigned)p.B);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = (size_t)AREA<D, NT> + (size_t)(p.chunk + STEP<D>) * sizeof(SlabEntry);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  if constexpr (CLUSTER) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)p.splits, 1, 1};
+    cfg.numAttrs = 1;
+  }
+  cudaError_t e = cudaLaunchKernelEx(&cfg, attn_decode_kernel<D, NT, BF16, CLUSTER>, p);
+  if (!CLUSTER && e == cudaSuccess && p.splits > 1) {
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)(p.B * p.Hq));
-    cfg.blockDim = dim3(THREADS);
-    cfg.stream = stream;
-    cfg.attrs = attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, attn_decode_join_kernel<D, BF16>, p);
-    if (e == cudaSuccess) e = cudaGetLastError();
+    cfg.gridDim = dim3((unsigned)(p.B * p.Hq));
+    cfg.dynamicSmemBytes = 0;
+    // many chunks, hence few sequences: more threads, so that all of a row's loads are still ahead
+    if (p.splits > 32) {
+      cfg.blockDim = dim3(512);
+      e = cudaLaunchKernelEx(&cfg, attn_decode_join_kernel<D, BF16, 512>, p);
+    } else {
+      e = cudaLaunchKernelEx(&cfg, attn_decode_join_kernel<D, BF16, THREADS>, p);
+    }
   }
-  if (e != cudaSuccess) return fail(B200_ERR_CUDA, "attn decode launch: %s", cudaGetErrorString(e));
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(B200_ERR_CUDA, "attn decode launch: %s", cudaGetErrorString(e));
+  }
   return B200_OK;
 }
 
+template <int D, int NT, bool BF16>
+int launch_c(DeviceCtx* ctx, cudaStream_t stream, const DecodeParams& p, bool cluster) {
+  return cluster ? launch_t<D, NT, BF16, true>(ctx, stream, p) : launch_t<D, NT, BF16, false>(ctx, stream, p);
+}
+
 template <bool BF16>
-int launch_d(DeviceCtx* ctx, cudaStream_t stream, const DecodeParams& p, int D, int nt) {
-  if (D == 64) return nt == 2 ? launch_t<64, 2, BF16>(ctx, stream, p) : launch_t<64, 1, BF16>(ctx, stream, p);
-  if (D == 128) return nt == 2 ? launch_t<128, 2, BF16>(ctx, stream, p) : launch_t<128, 1, BF16>(ctx, stream, p);
-  return launch_t<256, 1, BF16>(ctx, stream, p);
+int launch_d(DeviceCtx* ctx, cudaStream_t stream, const DecodeParams& p, int D, const DecodePlan& pl) {
+  if (D == 64) return pl.nt == 2 ? launch_c<64, 2, BF16>(ctx, stream, p, pl.cluster) : launch_c<64, 1, BF16>(ctx, stream, p, pl.cluster);
+  if (D == 128) return pl.nt == 2 ? launch_c<128, 2, BF16>(ctx, stream, p, pl.cluster) : launch_c<128, 1, BF16>(ctx, stream, p, pl.cluster);
+  return launch_c<256, 1, BF16>(ctx, stream, p, pl.cluster);
 }
 
 }  // namespace
 
 size_t attn_decode_workspace_bytes(int B, int Hq, int Hkv, int D, int page_size, int max_pages) {
   const DecodePlan pl = decode_plan(B, Hq, Hkv, D, page_size, max_pages);
-  return pl.splits > 1 ? (size_t)B * Hq * pl.splits * (D + 1) * sizeof(float) : 0;
+  return pl.splits > 1 && !pl.cluster ? (size_t)B * Hq * pl.splits * (D + 1) * sizeof(float) : 0;
 }
 
 int launch_attn_decode(DeviceCtx* ctx, cudaStream_t stream, const AttnDecodeArgs& a) {
@@ -656,7 +757,7 @@ int launch_attn_decode(DeviceCtx* ctx, cudaStream_t stream, const AttnDecodeArgs
   p.chunk = pl.chunk; p.splits = pl.splits;
   p.ws_o = a.workspace;
   p.ws_lse = a.workspace ? a.workspace + (size_t)a.B * a.Hq * pl.splits * a.c.D : nullptr;
-  return a.dtype == B200_BF16 ? launch_d<true>(ctx, stream, p, a.c.D, pl.nt) : launch_d<false>(ctx, stream, p, a.c.D, pl.nt);
+  return a.dtype == B200_BF16 ? launch_d<true>(ctx, stream, p, a.c.D, pl) : launch_d<false>(ctx, stream, p, a.c.D, pl);
 }
 
 }  // namespace tb
