@@ -303,8 +303,8 @@ B200_API int b200_attention_varlen_fwd(b200_stream_t stream, const void* q, cons
  * which become its last tokens.  The scale of a page and head is 2^e, e the smallest integer >= -126 with
  * |x| <= 448 * 2^e for every finite x of the rows written to it, raised (and the rows held already rounded
  * anew) when later rows need more; a row is stored as e4m3(x / scale), round to nearest even; values that are
- * not finite are stored as NaN.  A page that gets its row 0 starts a new scale.  Pages that two sequences
- * of one call write to are the caller's mistake (the result is one of the two, or a mixture). */
+ * not finite are stored as NaN.  A page that gets its row 0 starts a new scale.  A page that is named twice
+ * among those that a call writes to is the caller's mistake (the result is one of the two, or a mixture). */
 B200_API int b200_kv_append(b200_stream_t stream, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
                             int pages, int page_size, const int* page_table, int64_t table_stride, int max_pages,
                             const int* seq_lens, const void* k, const void* v, const int* cu_seqlens, int batch, int T,
@@ -313,7 +313,8 @@ B200_API int b200_kv_append(b200_stream_t stream, void* k_cache, void* v_cache, 
 /* Attention of one token per sequence over the cache: q, o [batch, Hq, D] of `dtype` (F16 or BF16, strides
  * {sequence, head, d}, multiples of 8 but for d), over the first seq_lens[b] tokens of sequence b (cut at
  * max_pages * page_size).  m (may be NULL): [batch, Hq] fp32, base-2 log-sum-exp.  A sequence without tokens
- * gives zeros and -inf.  `workspace`: b200_attention_decode_workspace(...) bytes (0: none needed), 16-byte
+ * gives zeros and -inf.  The launch covers max_pages * page_size tokens of every sequence (the lengths are
+ * not known on the host): pass no more columns of the table than the longest sequence needs.  `workspace`: b200_attention_decode_workspace(...) bytes (0: none needed), 16-byte
  * aligned, the caller's scratch for the call; calls that may overlap need one each.  Bitwise repeatable. */
 B200_API size_t b200_attention_decode_workspace(int batch, int Hq, int Hkv, int D, int page_size, int max_pages);
 B200_API int b200_attention_decode(b200_stream_t stream, const void* q, const void* k_cache, const void* v_cache,

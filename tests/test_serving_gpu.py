@@ -643,3 +643,88 @@ def test_custom_ops_run():
     assert torch.equal(a.k.view(torch.uint8), b.k.view(torch.uint8)) and torch.equal(a.v_scale, b.v_scale)
     x = torch.randn(2, 4, 64, device=DEV).half()
     assert torch.equal(ns.attention_decode(x, b.k, b.v, b.k_scale, b.v_scale, table, lens, 0.125), a.attend(x, table, lens, 0.125))
+
+
+def test_inputs_that_require_grad_under_no_grad():
+    q, k, v, cu, off = pack([33], 2, 1, 64, torch.float16, seed=71)
+    want = tb.attention_varlen(q, k, v, cu, True, 0.125)
+    q.requires_grad_(True)
+    with pytest.raises(RuntimeError, match="no backward"):
+        tb.attention_varlen(q, k, v, cu, True, 0.125)
+    with torch.no_grad():
+        assert torch.equal(tb.attention_varlen(q, k, v, cu, True, 0.125), want)
+
+
+def test_empty_batches_tables_and_caches():
+    c = tb.PagedKVCache(4, 16, 2, 64)
+    x = lambda *s: torch.randn(*s, device=DEV).half()
+    none = torch.zeros(0, dtype=I32, device=DEV)
+    assert c.attend(x(0, 4, 64), none.view(0, 3), none, 0.1).shape == (0, 4, 64)          # no sequence
+    c.append(x(0, 2, 64), x(0, 2, 64), none.view(0, 3), none)
+    o, M = c.attend(x(3, 4, 64), none.view(3, 0), ints(5, 0, 70), 0.1, return_stats=True)  # a table without a column
+    assert (o == 0).all() and (M == -math.inf).all()
+    c.append(x(3, 2, 64), x(3, 2, 64), none.view(3, 0), ints(5, 1, 70))
+    assert (c.k.view(torch.uint8) == 0).all() and (c.k_scale == 1).all()
+    e = tb.PagedKVCache(0, 16, 2, 64)                                                      # a cache without a page
+    table = torch.zeros(3, 2, dtype=I32, device=DEV)
+    e.append(x(3, 2, 64), x(3, 2, 64), table, ints(1, 2, 3))
+    assert (e.attend(x(3, 4, 64), table, ints(1, 2, 3), 0.1) == 0).all()
+
+
+@pytest.mark.parametrize("D,group,lens", [(128, 4, [20000, 3, 15001]), (64, 1, [5000] * 30), (256, 2, [9000, 0])])
+def test_decode_captured_where_chunks_are_joined_by_a_second_kernel(D, group, lens):
+    """Wide tables: the chunks' results go through a workspace.  Two graphs and eager calls in turn on streams of
+    their own give what each gives alone."""
+    c, table = filled_cache(lens, 2, 64, D, seed=D)
+    assert _lib.lib().b200_attention_decode_workspace(len(lens), 2 * group, 2, D, 64, table.shape[1]) > 0
+    g = torch.Generator(device=DEV).manual_seed(8)
+    qs = [torch.randn(len(lens), 2 * group, D, generator=g, device=DEV).half() for _ in range(3)]
+    n = torch.tensor(lens, dtype=I32, device=DEV)
+    want = [c.attend(q, table, n, 0.1, return_stats=True) for q in qs]
+    torch.cuda.synchronize()
+    check_decode(*want[0], qs[0], c, table, lens, 0.1)
+    streams, graphs, outs = [torch.cuda.Stream() for _ in qs], [], []
+    for q, st in zip(qs[:2], streams):
+        st.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=st):
+            outs.append(c.attend(q, table, n, 0.1, return_stats=True))
+        graphs.append(graph)
+    for _ in range(10):
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+        with torch.cuda.stream(streams[2]):
+            eager = c.attend(qs[2], table, n, 0.1, return_stats=True)
+        torch.cuda.synchronize()
+        for got, w in zip(outs + [eager], want):
+            assert torch.equal(got[0], w[0]) and torch.equal(got[1], w[1])
+
+
+def test_decode_table_sliced_to_the_longest_sequence():
+    """A table as wide as the longest sequence a program admits, its columns sliced to the ones in use."""
+    lens = [700, 12, 350]
+    c, table = filled_cache(lens, 2, 16, 128, seed=81)
+    wide = torch.full((3, 4096), -1, dtype=I32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    q = torch.randn(3, 6, 128, device=DEV).bfloat16()
+    n = torch.tensor(lens, dtype=I32, device=DEV)
+    o = c.attend(q, wide[:, :table.shape[1]], n, 0.1)
+    assert torch.equal(o, c.attend(q, table, n, 0.1))
+    o2, M2 = c.attend(q, wide, n, 0.1, return_stats=True)
+    check_decode(o2, M2, q, c, table, lens, 0.1)
+
+
+def test_decode_a_sequence_does_not_depend_on_the_others():
+    """Its bits are those of the sequence alone under a table of the same width and a batch of the same size."""
+    lens = [1500, 900, 40, 1501]
+    c, table = filled_cache(lens, 2, 32, 64, seed=82)
+    q = torch.randn(4, 8, 64, device=DEV).half()
+    n = torch.tensor(lens, dtype=I32, device=DEV)
+    o = c.attend(q, table, n, 0.1)
+    for b in range(4):
+        only = torch.zeros_like(n)
+        only[b] = n[b]
+        other = torch.full_like(table, -1)
+        other[b] = table[b]
+        assert torch.equal(c.attend(q, other, only, 0.1)[b], o[b])

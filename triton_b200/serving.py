@@ -52,9 +52,7 @@ def kv_cache_append(k_cache, v_cache, k_scale, v_scale, k, v, page_table, seq_le
     row per sequence without cu_seqlens (T == batch).
     The scale of a page and head is a power of two, 2^e with the smallest e >= -126 that lets e4m3's 448 * 2^e
     reach every finite value; values are stored as x / scale rounded to nearest even, non-finite ones as NaN.
-    When later rows need a larger scale the page's earlier rows are rounded to it.  The stored bytes depend on
-    nothing else.  Two sequences of one call may not write to the same page.
-    """
+  XX    """
     (_lib._binding or _lib.binding()).kv_cache_append(k_cache, v_cache, k_scale, v_scale, k, v, page_table, seq_lens, cu_seqlens)
 
 
@@ -62,7 +60,9 @@ def attention_decode(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens
     """Attention of one token per sequence over the paged cache: q [batch, Hq, D] in fp16 or bf16, Hq a multiple
     of the cache's heads, over the first seq_lens[b] tokens (the new one among them, once it is appended).  Tokens
     of a page that the table does not name are left out; a sequence without tokens gives zeros.  Returns O like
-    q, with return_stats=True (O, M): M [batch, Hq] is the base-2 log-sum-exp (-inf without tokens)."""
+    q, with return_stats=True (O, M): M [batch, Hq] is the base-2 log-sum-exp (-inf without tokens).
+    The lengths stay on the GPU, so the launch covers what the table has room for: where that is far more than
+    the longest sequence, pass its first columns (page_table[:, :n])."""
     return (_lib._binding or _lib.binding()).attention_decode(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, sm_scale,
                                                               out, return_stats)
 
