@@ -728,3 +728,19 @@ def test_decode_a_sequence_does_not_depend_on_the_others():
         other = torch.full_like(table, -1)
         other[b] = table[b]
         assert torch.equal(c.attend(q, other, only, 0.1)[b], o[b])
+
+
+def test_varlen_a_very_large_batch():
+    """40000 sequences of 0 to 3 rows: finding the items stays linear in them."""
+    lens = [i % 4 for i in range(40000)]
+    q, k, v, cu, off = pack(lens, 2, 1, 64, torch.float16, seed=91)
+    o = tb.attention_varlen(q, k, v, cu, True, 0.125)
+    first = torch.tensor([off[b] for b in range(40000) if lens[b]], device=DEV)
+    assert torch.equal(o[first], v[first].expand(-1, 2, -1))  # a first row sees itself alone
+    second = torch.tensor([off[b] + 1 for b in range(40000) if lens[b] >= 2], device=DEV)
+    with_first = (q[second].double() * k[second - 1].double()).sum(-1) * 0.125
+    own = (q[second].double() * k[second].double()).sum(-1) * 0.125
+    p = torch.softmax(torch.stack([with_first, own], -1), -1)
+    want = p[..., :1] * v[second - 1].double() + p[..., 1:] * v[second].double()
+    bound = 2.0 ** -11 * want.abs() + (2.0 ** -11 + 2.0 ** -12 + 2.0 ** -14) * (v[second - 1].double().abs() + v[second].double().abs())
+    assert bool(((o[second].double() - want).abs() <= bound).all())

@@ -158,6 +158,7 @@ __device__ __forceinline__ Item decode_item(const FwdParams& p, int w) {
 template <int ROWS>
 struct PackedWalk {
   int blocks, base, count, total;  // the class: query blocks, its first ticket, sequences in it
+  int at, before;                  // where the last draw's search ended: 32 sequences from `at`, `before` of the class before them
   bool by_level;
 
   static __device__ __forceinline__ void extent(const PackedFwdParams& p, int b, int& start, int& len) {
@@ -182,6 +183,7 @@ struct PackedWalk {
     blocks = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);
     for (int b = lane; b < p.batch; b += 32) c += in_class(seq_blocks(p, b));
     count = blocks > 0 ? (int)__reduce_add_sync(0xffffffffu, (unsigned)c) : 0;
+    at = before = 0;
   }
   __device__ __forceinline__ void init(const PackedFwdParams& p) {
     by_level = p.by_level;
@@ -206,14 +208,13 @@ struct PackedWalk {
     it.h = it.kh * p.group + r % p.group;
     it.z = it.zh = 0;
     it.row0 = it.N = 0;
-    int before = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += 32) {
-      const int b = b0 + lane;
+    for (; at < p.batch; at += 32) {
+      const int b = at + lane;
       const unsigned in = __ballot_sync(0xffffffffu, b < p.batch && in_class(seq_blocks(p, b)));
       const int here = __popc(in);
       if (nth < before + here) {
         const bool me = ((in >> lane) & 1u) && __popc(in & ((1u << lane) - 1u)) == nth - before;
-        extent(p, b0 + __ffs(__ballot_sync(0xffffffffu, me)) - 1, it.row0, it.N);
+        extent(p, at + __ffs(__ballot_sync(0xffffffffu, me)) - 1, it.row0, it.N);
         break;
       }
       before += here;
