@@ -269,15 +269,30 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
   }
   const uint8_t* room_k = smem + warp * ROOM<D>;
   const uint8_t* room_v = room_k + SL * SIDE;
-  auto fetch = [&](int i, const uint8_t* dst, const uint8_t* src) {
+  SlabEntry ahead[SL];  // the step whose bytes are being sent for
+  auto look = [&](int i) {
+#pragma unroll
+    for (int u = 0; u < SL; ++u) ahead[u] = SlabEntry{~0u, 0u};
+    if (i < count) {
+      if constexpr (SL == 2) {
+        const uint4 e = *reinterpret_cast<const uint4*>(table + i);
+        ahead[0] = SlabEntry{e.x, e.y};
+        ahead[1] = SlabEntry{e.z, e.w};
+      } else {
+        ahead[0] = table[i];
+      }
+    }
+  };
+  auto fetch = [&](const uint8_t* dst, const uint8_t* src) {
 #pragma unroll
     for (int u = 0; u < SL; ++u)
-      if (i + u < count && table[i + u].slab != ~0u) fetch_slab<D>(smem_u32(dst) + u * SIDE, src, table[i + u].slab, lane);
+      if (ahead[u].slab != ~0u) fetch_slab<D>(smem_u32(dst) + u * SIDE, src, ahead[u].slab, lane);
     cp_async_commit();
   };
   __syncthreads();
-  fetch(warp * SL, room_k, p.k);
-  fetch(warp * SL, room_v, p.v);
+  look(warp * SL);
+  fetch(room_k, p.k);
+  fetch(room_v, p.v);
   for (int i = threadIdx.x; i < count; i += THREADS)
     if (table[i].slab != ~0u) {
       const unsigned ph = table[i].slab >> sh;
@@ -337,19 +352,20 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
   int seen = 0;
 
   __syncthreads();
+  look(warp * SL);  // with the scales
   for (int i = warp * SL; i < count; i += WARPS * SL) {
-    const int next = i + WARPS * SL;
     float ks[SL], ev[SL];
     int left[SL];  // tokens of the slab that exist
     bool any_here = false;
 #pragma unroll
     for (int u = 0; u < SL; ++u) {
-      const SlabEntry e = table[i + u];
+      const SlabEntry e = ahead[u];
       ks[u] = __uint_as_float((e.scales & 0xFFu) << 23);
-      ev[u] = (float)((int)(e.scales >> 8 & 0xFFu) - 127);
+      ev[u] = __uint_as_float(0x4B000000u | (e.scales >> 8 & 0xFFu)) - (8388608.f + 127.f);  // the field as a number, less its bias
       left[u] = e.slab != ~0u ? len - (s0 + i + u) * SLAB : 0;
       any_here |= e.slab != ~0u;
     }
+    look(i + WARPS * SL);
     float s[SL][NT][4];
     cp_async_wait<1>();  // K is here, V may be under way
     __syncwarp();
@@ -375,7 +391,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
         }
     }
     __syncwarp();
-    fetch(next, room_k, p.k);
+    fetch(room_k, p.k);
     uint32_t pb[SL][NT][2];
     if (any_here) {
       seen = 1;
@@ -482,7 +498,7 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
       }
     }
     __syncwarp();
-    fetch(next, room_v, p.v);
+    fetch(room_v, p.v);
   }
   cp_async_wait<0>();
 
