@@ -744,3 +744,27 @@ def test_varlen_a_very_large_batch():
     want = p[..., :1] * v[second - 1].double() + p[..., 1:] * v[second].double()
     bound = 2.0 ** -11 * want.abs() + (2.0 ** -11 + 2.0 ** -12 + 2.0 ** -14) * (v[second - 1].double().abs() + v[second].double().abs())
     assert bool(((o[second].double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("hq,hkv,D", [(16, 8, 64), (24, 4, 128), (32, 1, 128)])
+def test_varlen_short_sequences_two_heads_to_an_item(hq, hkv, D, causal):
+    """Enough short sequences, an even number of heads per k/v head: an item is 128 rows of two heads."""
+    lens = [1, 127, 128, 129, 300, 5, 0, 640, 77, 256] + [(13 * i) % 200 for i in range(60)]
+    q, k, v, cu, off = pack(lens, hq, hkv, D, torch.bfloat16, seed=hq + D, tail=9)
+    assert q.shape[0] <= 640 * len(lens) and (q.shape[0] // 128 + len(lens)) * hq // 2 >= 148
+    o, M = tb.attention_varlen(q, k, v, cu, causal, 0.1, return_stats=True)
+    some = list(range(0, hq, 5)) + [hq - 1]
+    for b in list(range(10)) + [33, 69]:
+        a, e = off[b], off[b + 1]
+        for h in some if e > a else []:
+            kh = h // (hq // hkv)
+            want = one_head(q[a:e, h], k[a:e, kh], v[a:e, kh], 0.1, causal)
+            check(o[a:e, h], want, q.dtype, q.dtype, f"sequence {b} head {h}")
+            check_lse(M[h, a:e], want, f"lse of sequence {b} head {h}")
+    # every sequence and head against the one that takes 256 rows of a head (few items)
+    for b in range(0, 70, 7):
+        a, e = off[b], off[b + 1]
+        if a < e:
+            assert torch.equal(o[a:e], tb.attention_varlen(q[a:e], k[a:e], v[a:e], ints(0, e - a), causal, 0.1))
+    assert (o[off[-1]:] == 0).all()

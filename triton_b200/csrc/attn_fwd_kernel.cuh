@@ -33,7 +33,8 @@
 // of 128, and what it reads of the next sequence is masked by the length as the ragged end of a dense
 // batch is; the rows of V behind the end are cleared in shared memory before the MMA (they are another
 // sequence's: 0 * inf would reach this one).  The scheduling warp finds the item of a ticket from cu
-// (PackedWalk) and publishes it, so the lengths are never needed on the host.
+// (PackedWalk) and publishes it, so the lengths are never needed on the host.  With an even number
+// of heads per k/v head an item's two tiles can also be the same 128 rows of two of them (`pair`).
 // TMEM columns: S0 [0,128) S1 [128,256) O0 [256,256+D) O1 [384,384+D); P_i = first 64 columns of S_i
 // at head dim 128, and columns [320,384) / [448,512) at head dim 64 (16-bit), where S_i of the next
 // block is then issued before P_i V of this one.  Head dim 256: S [0,128), O [256,512).
@@ -88,6 +89,7 @@ struct PackedFwdParams : FwdParams {
   const int* cu;    // [batch + 1] offsets into the T rows (N = T, Z = 1, H = Hq)
   int batch, group;  // group: query heads per k/v head
   int by_level;      // order of the items, see PackedWalk
+  int pair;          // an item's two tiles are 1: the same 128 rows of two heads of a group, 0: 256 rows of one head
   int zero_rest;     // rows of o that belong to no sequence: 0 left as they are, 1 set to zero
 };
 
@@ -125,8 +127,12 @@ struct Item {
   int row0, kh, N;                 // first row of the sequence in the tensors, k/v head, length
 };
 template <int TILES>
-__device__ __forceinline__ void count_blocks(Item& it, bool causal) {
+__device__ __forceinline__ void count_blocks(Item& it, bool causal, bool pair = false) {
   const int nkv_all = (it.N + BLK - 1) / BLK;
+  if (pair) {  // both tiles see the same blocks
+    it.n0 = it.n1 = it.nmax = causal ? min(it.qb + 1, nkv_all) : nkv_all;
+    return;
+  }
   // K/V blocks per tile: up to and including the block that holds the tile's diagonal when causal
   it.n0 = causal ? min(TILES * it.qb + 1, nkv_all) : nkv_all;
   it.n1 = (TILES == 2) ? (causal ? min(2 * it.qb + 2, nkv_all) : nkv_all) : 0;  // n0 <= n1 <= n0 + 1 with two tiles
@@ -155,23 +161,23 @@ __device__ __forceinline__ Item decode_item(const FwdParams& p, int w) {
 //              the items that read the same K and V follow one another, which is what counts when the pack's
 //              K and V do not stay in L2.
 // Warp-collective.  Offsets outside [0, T] and negative lengths are cut, so none can lead out of the tensors.
-template <int ROWS>
 struct PackedWalk {
   int blocks, base, count, total;  // the class: query blocks, its first ticket, sequences in it
   int at, before;                  // where the last draw's search ended: 32 sequences from `at`, `before` of the class before them
+  int rows, heads, group;          // of an item: query rows; items per block (heads, or pairs of them), and per k/v head
   bool by_level;
 
   static __device__ __forceinline__ void extent(const PackedFwdParams& p, int b, int& start, int& len) {
     start = min(max(__ldg(p.cu + b), 0), p.N);
     len = max(min(__ldg(p.cu + b + 1), p.N) - start, 0);
   }
-  static __device__ __forceinline__ int seq_blocks(const PackedFwdParams& p, int b) {
+  __device__ __forceinline__ int seq_blocks(const PackedFwdParams& p, int b) const {
     int start, len;
     extent(p, b, start, len);
-    return (len + ROWS - 1) / ROWS;
+    return (len + rows - 1) / rows;
   }
   __device__ __forceinline__ bool in_class(int n) const { return by_level ? n >= blocks : n == blocks; }
-  __device__ __forceinline__ int tickets(const PackedFwdParams& p) const { return count * p.H * (by_level ? 1 : blocks); }
+  __device__ __forceinline__ int tickets() const { return count * heads * (by_level ? 1 : blocks); }
   // the class of the most blocks below `below`
   __device__ __forceinline__ void enter(const PackedFwdParams& p, int below) {
     const int lane = threadIdx.x & 31;
@@ -185,27 +191,30 @@ struct PackedWalk {
     count = blocks > 0 ? (int)__reduce_add_sync(0xffffffffu, (unsigned)c) : 0;
     at = before = 0;
   }
-  __device__ __forceinline__ void init(const PackedFwdParams& p) {
+  __device__ __forceinline__ void init(const PackedFwdParams& p, int item_rows) {
     by_level = p.by_level;
+    rows = p.pair ? BLK : item_rows;
+    heads = p.pair ? p.H / 2 : p.H;
+    group = p.pair ? p.group / 2 : p.group;
     int sum = 0;
     for (int b = threadIdx.x & 31; b < p.batch; b += 32) sum += seq_blocks(p, b);
-    total = (int)__reduce_add_sync(0xffffffffu, (unsigned)sum) * p.H;
+    total = (int)__reduce_add_sync(0xffffffffu, (unsigned)sum) * heads;
     base = 0;
     enter(p, 0x7fffffff);
   }
   __device__ __forceinline__ Item find(const PackedFwdParams& p, int w) {  // w < total
-    while (blocks > 0 && w - base >= tickets(p)) {
-      base += tickets(p);
+    while (blocks > 0 && w - base >= tickets()) {
+      base += tickets();
       enter(p, blocks);
     }
-    const int lane = threadIdx.x & 31, per_seq = p.H * (by_level ? 1 : blocks), per_kv = p.group * (by_level ? 1 : blocks);
+    const int lane = threadIdx.x & 31, per_seq = heads * (by_level ? 1 : blocks), per_kv = group * (by_level ? 1 : blocks);
     const int nth = (w - base) / per_seq;
     int r = (w - base) - nth * per_seq;
     Item it;
     it.kh = r / per_kv;
     r -= it.kh * per_kv;
-    it.qb = blocks - 1 - r / p.group;  // (by level r < group)
-    it.h = it.kh * p.group + r % p.group;
+    it.qb = blocks - 1 - r / group;  // (by level r < group)
+    it.h = it.kh * p.group + r % group * (p.pair ? 2 : 1);
     it.z = it.zh = 0;
     it.row0 = it.N = 0;
     for (; at < p.batch; at += 32) {
@@ -256,6 +265,15 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   // [2] ticket; packed: [2][8] ticket (-1: none left), query block, head, first row, length
   volatile int* sched_item = reinterpret_cast<volatile int*>(tmem_slot + 2);
   constexpr int SLOT = PACKED ? 8 : 1;
+  // first row of tile i in its sequence, and its head
+  auto tile_row0 = [&](const Item& it, int i) {
+    if constexpr (PACKED) return p.pair ? it.qb * BLK : it.qb * ITEM_ROWS + i * BLK;
+    else return it.qb * ITEM_ROWS + i * BLK;
+  };
+  auto tile_head = [&](const Item& it, int i) {
+    if constexpr (PACKED) return it.h + (p.pair ? i : 0);
+    else return it.h;
+  };
   // the item that a published slot names, for the warps that read it; false: no item is left
   auto take_item = [&](int slot, int w, Item& it) {
     if constexpr (PACKED) {
@@ -265,7 +283,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       it.N = sched_item[8 * slot + 4];
       it.z = it.zh = 0;
       it.kh = it.h / p.group;
-      count_blocks<TILES>(it, p.causal);
+      count_blocks<TILES>(it, p.causal, p.pair);
       return w >= 0;
     } else {
       if (w >= p.total_items) return false;
@@ -363,7 +381,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       mbar_wait<WAIT_PAUSE>(q_empty, (n & 1u) ^ 1u, p.status, SITE_FWD_Q);  // previous item's S MMAs are done with Q
       for (int i = 0; i < TILES; ++i) {
         mbar_expect_tx(&q_full[i], TILE);
-        load_tile<D, FP8>(sq + i * TILE, &tm_q, &q_full[i], it.row0 + it.qb * ITEM_ROWS + i * BLK, it.h, it.z);
+        load_tile<D, FP8>(sq + i * TILE, &tm_q, &q_full[i], it.row0 + tile_row0(it, i), tile_head(it, i), it.z);
       }
       for (int j = 0; j < it.nmax; ++j) {
         for (int kv = 0; kv < 2; ++kv) {  // K_j then V_j
@@ -375,8 +393,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       }
     };
     if constexpr (PACKED) {
-      PackedWalk<ITEM_ROWS> walk;
-      walk.init(p);
+      PackedWalk walk;
+      walk.init(p, ITEM_ROWS);
       for (uint32_t n = 0;; ++n) {
         int w = 0;
         if (lane == 0) w = atomicAdd(p.sched_counter, 1);
@@ -384,7 +402,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         const bool more = w < walk.total;
         Item it{};
         if (more) it = walk.find(p, w);
-        count_blocks<TILES>(it, p.causal);
+        count_blocks<TILES>(it, p.causal, p.pair);
         if (lane == 0) {
           const uint32_t slot = n & 1u, sph = (n >> 1) & 1u;
           mbar_wait<WAIT_PAUSE>(&sched_empty[slot], sph ^ 1u, p.status, SITE_FWD_SCHED);
@@ -622,9 +640,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         w = __shfl_sync(0xffffffffu, w, 0);
         if (!take_item(slot, w, it)) break;
       }
-      const int qb = it.qb;
+      const int row0 = tile_row0(it, i), head = tile_head(it, i);
       const int N = PACKED ? it.N : p.N;
-      const int row = qb * ITEM_ROWS + i * BLK + row_in_tile;  // query index
+      const int row = row0 + row_in_tile;  // query index
       const int nb = i ? it.n1 : it.n0;
       float m_ref = -INFINITY, l = 0.f;
       float m_true = -INFINITY;  // the exact running maximum (m_ref lags it by up to the rescale threshold)
@@ -636,7 +654,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         if (traced) B200_TRACE_EVENT(p.status, i, 1);
         tc_fence_after();
         const int col0 = j * BLK;
-        const bool need_mask = (p.causal && col0 + BLK - 1 > qb * ITEM_ROWS + i * BLK) || (col0 + BLK > N);
+        const bool need_mask = (p.causal && col0 + BLK - 1 > row0) || (col0 + BLK > N);
         // load 32 columns at a time; the row maximum of a chunk is taken while the next chunk loads
         uint32_t r[BLK];
         float mx4[16];
@@ -781,16 +799,16 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       tc_fence_after();
       const float inv_l = 1.f / l;
       const bool valid = row < N;
-      uint16_t* orow = reinterpret_cast<uint16_t*>(p.o) + (long long)it.z * p.o_sz + (long long)it.h * p.o_sh +
+      uint16_t* orow = reinterpret_cast<uint16_t*>(p.o) + (long long)it.z * p.o_sz + (long long)head * p.o_sh +
                        (long long)(it.row0 + row) * p.o_sn;
       // packed: a box that reaches past the sequence's end would overwrite the next one
-      if (p.o_tma && (!PACKED || qb * ITEM_ROWS + i * BLK + (int)quarter * 32 + 32 <= N)) {
+      if (p.o_tma && (!PACKED || row0 + (int)quarter * 32 + 32 <= N)) {
         // 64 columns at a time: scaled, packed, written to this warp's swizzled staging buffer and
         // stored by TMA (full 128-byte lines; rows past N are clipped by the hardware).  A warp-wide
         // store of one row per lane touches 32 lines per instruction and made this epilogue cost
         // 5200 clk per item at D = 128.
         uint8_t* stg = sstage + warp * Cfg::STG_BYTES;
-        const int warp_row0 = qb * ITEM_ROWS + i * BLK + quarter * 32;
+        const int warp_row0 = row0 + quarter * 32;
         if constexpr (FP8) {
           // 8-bit O: the D columns of a row are one line of the staging buffer
           if (lane == 0) tma_store_wait_read<0>();
@@ -815,7 +833,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0 && warp_row0 < N) {
-            tma_store_4d(&tm_o_map, stg, 0, warp_row0, it.h, it.z);
+            tma_store_4d(&tm_o_map, stg, 0, warp_row0, head, it.z);
             tma_store_commit();
           }
         } else
@@ -841,7 +859,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           __syncwarp();
           if (traced) B200_TRACE_EVENT(p.status, i, 0xC);
           if (lane == 0 && warp_row0 < N) {
-            tma_store_4d(&tm_o_map, stg, c, it.row0 + warp_row0, it.h, it.z);
+            tma_store_4d(&tm_o_map, stg, c, it.row0 + warp_row0, head, it.z);
             tma_store_commit();
           }
         }
@@ -880,7 +898,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
       }
       if constexpr (PACKED) {
-        if (valid && p.m) p.m[(long long)it.h * p.N + it.row0 + row] = m_ref + log2f(l);
+        if (valid && p.m) p.m[(long long)head * p.N + it.row0 + row] = m_ref + log2f(l);
       } else if (valid) {
         p.m[(long long)it.zh * p.N + row] = m_ref + log2f(l);
       }
