@@ -165,13 +165,15 @@ struct PackedWalk {
   int blocks, base, count, total;  // the class: query blocks, its first ticket, sequences in it
   int at, before;                  // where the last draw's search ended: 32 sequences from `at`, `before` of the class before them
   int rows, heads, group;          // of an item: query rows; items per block (heads, or pairs of them), and per k/v head
+  int start0, len0, blocks0;       // of sequence `lane`: most batches need no more than this one load
   bool by_level;
 
   static __device__ __forceinline__ void extent(const PackedFwdParams& p, int b, int& start, int& len) {
     start = min(max(__ldg(p.cu + b), 0), p.N);
     len = max(min(__ldg(p.cu + b + 1), p.N) - start, 0);
   }
-  __device__ __forceinline__ int seq_blocks(const PackedFwdParams& p, int b) const {
+  __device__ __forceinline__ int seq_blocks(const PackedFwdParams& p, int b) const {  // b = lane + 32 i
+    if (b < 32) return blocks0;
     int start, len;
     extent(p, b, start, len);
     return (len + rows - 1) / rows;
@@ -196,6 +198,9 @@ struct PackedWalk {
     rows = p.pair ? BLK : item_rows;
     heads = p.pair ? p.H / 2 : p.H;
     group = p.pair ? p.group / 2 : p.group;
+    start0 = len0 = 0;
+    if ((int)(threadIdx.x & 31) < p.batch) extent(p, threadIdx.x & 31, start0, len0);
+    blocks0 = (len0 + rows - 1) / rows;
     int sum = 0;
     for (int b = threadIdx.x & 31; b < p.batch; b += 32) sum += seq_blocks(p, b);
     total = (int)__reduce_add_sync(0xffffffffu, (unsigned)sum) * heads;
@@ -223,7 +228,10 @@ struct PackedWalk {
       const int here = __popc(in);
       if (nth < before + here) {
         const bool me = ((in >> lane) & 1u) && __popc(in & ((1u << lane) - 1u)) == nth - before;
-        extent(p, at + __ffs(__ballot_sync(0xffffffffu, me)) - 1, it.row0, it.N);
+        const int src = __ffs(__ballot_sync(0xffffffffu, me)) - 1;
+        it.row0 = __shfl_sync(0xffffffffu, start0, src);
+        it.N = __shfl_sync(0xffffffffu, len0, src);
+        if (at > 0) extent(p, at + src, it.row0, it.N);
         break;
       }
       before += here;
