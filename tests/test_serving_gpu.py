@@ -479,6 +479,12 @@ def test_decode_queries_far_from_one():
         o, M = c.attend((q.double() * 2.0 ** e).bfloat16(), table, ints(200), scale, return_stats=True)
         o0, M0 = c.attend(q, table, ints(200), 0.125, return_stats=True)
         assert torch.equal(o, o0) and torch.equal(M, M0)
+    # near the end of bf16's range, with values that stay normal numbers there
+    q = ((1 + torch.rand(1, 4, 64, device=DEV, generator=g)) * torch.randn(1, 4, 64, device=DEV, generator=g).sign()).bfloat16()
+    for e, scale in ((-118, 2.0 ** 115), (-125, 2.0 ** 122), (120, 2.0 ** -123)):
+        o, M = c.attend((q.double() * 2.0 ** e).bfloat16(), table, ints(200), scale, return_stats=True)
+        o0, M0 = c.attend(q, table, ints(200), 0.125, return_stats=True)
+        assert torch.equal(o, o0) and torch.equal(M, M0)
     mixed = q.clone()
     mixed[0, 1] = (q[0, 1].double() * 2.0 ** -50).bfloat16()
     mixed[0, 3] = 0.0
