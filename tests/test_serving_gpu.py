@@ -753,12 +753,13 @@ def test_varlen_a_very_large_batch():
 
 
 @pytest.mark.parametrize("causal", [True, False])
-@pytest.mark.parametrize("hq,hkv,D", [(16, 8, 64), (24, 4, 128), (32, 1, 128)])
-def test_varlen_short_sequences_two_heads_to_an_item(hq, hkv, D, causal):
-    """Enough short sequences, an even number of heads per k/v head: an item is 128 rows of two heads."""
+@pytest.mark.parametrize("hq,hkv,D", [(16, 8, 64), (24, 4, 128), (32, 1, 128), (9, 3, 64), (21, 3, 256), (40, 1, 64), (26, 2, 128)])
+def test_varlen_short_sequences_all_heads_of_a_group_to_a_tile(hq, hkv, D, causal):
+    """Short sequences: a tile's rows are positions times the heads of a group (up to 32 of them), whether those
+    divide a warp's rows (2, 6, 32) or not (3, 7, 13); 40 heads stay one by one."""
     lens = [1, 127, 128, 129, 300, 5, 0, 640, 77, 256] + [(13 * i) % 200 for i in range(60)]
     q, k, v, cu, off = pack(lens, hq, hkv, D, torch.bfloat16, seed=hq + D, tail=9)
-    assert q.shape[0] <= 640 * len(lens) and (q.shape[0] // 128 + len(lens)) * hq // 2 >= 148
+    assert q.shape[0] <= 192 * len(lens)
     o, M = tb.attention_varlen(q, k, v, cu, causal, 0.1, return_stats=True)
     some = list(range(0, hq, 5)) + [hq - 1]
     for b in list(range(10)) + [33, 69]:
@@ -768,9 +769,18 @@ def test_varlen_short_sequences_two_heads_to_an_item(hq, hkv, D, causal):
             want = one_head(q[a:e, h], k[a:e, kh], v[a:e, kh], 0.1, causal)
             check(o[a:e, h], want, q.dtype, q.dtype, f"sequence {b} head {h}")
             check_lse(M[h, a:e], want, f"lse of sequence {b} head {h}")
-    # every sequence and head against the one that takes 256 rows of a head (few items)
+    # a short sequence's bits are those it has alone
     for b in range(0, 70, 7):
         a, e = off[b], off[b + 1]
-        if a < e:
+        if 0 < e - a <= 192:
             assert torch.equal(o[a:e], tb.attention_varlen(q[a:e], k[a:e], v[a:e], ints(0, e - a), causal, 0.1))
-    assert (o[off[-1]:] == 0).all()
+    assert (o[off[-1]:] == 0).all() and (M[:, off[-1]:] == -math.inf).all()
+    mine = torch.full_like(q, 5.0)
+    tb.attention_varlen(q, k, v, cu, causal, 0.1, out=mine)
+    assert torch.equal(mine[:off[-1]], o[:off[-1]]) and (mine[off[-1]:] == 5.0).all()
+    q[off[4]:off[5]] = math.nan  # neighbours stay as they are
+    k[off[4]:off[5]] = math.inf
+    v[off[4]:off[5]] = math.nan
+    v[off[-1]:] = math.nan
+    again = tb.attention_varlen(q, k, v, cu, causal, 0.1)
+    assert torch.equal(again[:off[4]], o[:off[4]]) and torch.equal(again[off[5]:], o[off[5]:])

@@ -33,8 +33,9 @@
 // of 128, and what it reads of the next sequence is masked by the length as the ragged end of a dense
 // batch is; the rows of V behind the end are cleared in shared memory before the MMA (they are another
 // sequence's: 0 * inf would reach this one).  The scheduling warp finds the item of a ticket from cu
-// (PackedWalk) and publishes it, so the lengths are never needed on the host.  With an even number
-// of heads per k/v head an item's two tiles can also be the same 128 rows of two of them (`pair`).
+// (PackedWalk) and publishes it, so the lengths are never needed on the host.  With several heads per
+// k/v head a tile can also be 128 / fold positions of all `fold` of them, row = position * fold + head: the
+// tensor map of q brings such a tile as one box, and the mask goes by the row's position.
 // TMEM columns: S0 [0,128) S1 [128,256) O0 [256,256+D) O1 [384,384+D); P_i = first 64 columns of S_i
 // at head dim 128, and columns [320,384) / [448,512) at head dim 64 (16-bit), where S_i of the next
 // block is then issued before P_i V of this one.  Head dim 256: S [0,128), O [256,512).
@@ -89,7 +90,8 @@ struct PackedFwdParams : FwdParams {
   const int* cu;    // [batch + 1] offsets into the T rows (N = T, Z = 1, H = Hq)
   int batch, group;  // group: query heads per k/v head
   int by_level;      // order of the items, see PackedWalk
-  int pair;          // an item's two tiles are 1: the same 128 rows of two heads of a group, 0: 256 rows of one head
+  int fold;          // heads of a tile: 1, or all of a group
+  int tile_pos;      // positions of a tile: 128 / fold
   int zero_rest;     // rows of o that belong to no sequence: 0 left as they are, 1 set to zero
 };
 
@@ -126,16 +128,13 @@ struct Item {
   int qb, zh, z, h, n0, n1, nmax;  // n_i: K/V blocks tile i visits; nmax: blocks the item streams
   int row0, kh, N;                 // first row of the sequence in the tensors, k/v head, length
 };
+// tile_pos: query positions of a tile
 template <int TILES>
-__device__ __forceinline__ void count_blocks(Item& it, bool causal, bool pair = false) {
-  const int nkv_all = (it.N + BLK - 1) / BLK;
-  if (pair) {  // both tiles see the same blocks
-    it.n0 = it.n1 = it.nmax = causal ? min(it.qb + 1, nkv_all) : nkv_all;
-    return;
-  }
-  // K/V blocks per tile: up to and including the block that holds the tile's diagonal when causal
-  it.n0 = causal ? min(TILES * it.qb + 1, nkv_all) : nkv_all;
-  it.n1 = (TILES == 2) ? (causal ? min(2 * it.qb + 2, nkv_all) : nkv_all) : 0;  // n0 <= n1 <= n0 + 1 with two tiles
+__device__ __forceinline__ void count_blocks(Item& it, bool causal, int tile_pos = BLK) {
+  const int nkv_all = (it.N + BLK - 1) / BLK, end0 = (TILES * it.qb + 1) * tile_pos, end1 = end0 + tile_pos;
+  // K/V blocks per tile: up to and including the block that holds the tile's last diagonal when causal
+  it.n0 = causal ? min((end0 + BLK - 1) / BLK, nkv_all) : nkv_all;
+  it.n1 = (TILES == 2) ? (causal ? min((end1 + BLK - 1) / BLK, nkv_all) : nkv_all) : 0;  // n0 <= n1 <= n0 + 1 with two tiles
   it.nmax = (TILES == 2) ? it.n1 : it.n0;
 }
 template <int TILES>
@@ -164,7 +163,7 @@ __device__ __forceinline__ Item decode_item(const FwdParams& p, int w) {
 struct PackedWalk {
   int blocks, base, count, total;  // the class: query blocks, its first ticket, sequences in it
   int at, before;                  // where the last draw's search ended: 32 sequences from `at`, `before` of the class before them
-  int rows, heads, group;          // of an item: query rows; items per block (heads, or pairs of them), and per k/v head
+  int rows, heads, group;          // positions of an item; items per block of positions, and of those per k/v head
   int start0, len0, blocks0;       // of sequence `lane`: most batches need no more than this one load
   bool by_level;
 
@@ -193,11 +192,11 @@ struct PackedWalk {
     count = blocks > 0 ? (int)__reduce_add_sync(0xffffffffu, (unsigned)c) : 0;
     at = before = 0;
   }
-  __device__ __forceinline__ void init(const PackedFwdParams& p, int item_rows) {
+  __device__ __forceinline__ void init(const PackedFwdParams& p, int tiles) {
     by_level = p.by_level;
-    rows = p.pair ? BLK : item_rows;
-    heads = p.pair ? p.H / 2 : p.H;
-    group = p.pair ? p.group / 2 : p.group;
+    rows = tiles * p.tile_pos;
+    heads = p.H / p.fold;
+    group = p.group / p.fold;
     start0 = len0 = 0;
     if ((int)(threadIdx.x & 31) < p.batch) extent(p, threadIdx.x & 31, start0, len0);
     blocks0 = (len0 + rows - 1) / rows;
@@ -219,7 +218,7 @@ struct PackedWalk {
     it.kh = r / per_kv;
     r -= it.kh * per_kv;
     it.qb = blocks - 1 - r / group;  // (by level r < group)
-    it.h = it.kh * p.group + r % group * (p.pair ? 2 : 1);
+    it.h = it.kh * p.group + r % group;  // (folded: group = 1, the first of the heads)
     it.z = it.zh = 0;
     it.row0 = it.N = 0;
     for (; at < p.batch; at += 32) {
@@ -273,14 +272,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   // [2] ticket; packed: [2][8] ticket (-1: none left), query block, head, first row, length
   volatile int* sched_item = reinterpret_cast<volatile int*>(tmem_slot + 2);
   constexpr int SLOT = PACKED ? 8 : 1;
-  // first row of tile i in its sequence, and its head
+  // first position of tile i in its sequence
   auto tile_row0 = [&](const Item& it, int i) {
-    if constexpr (PACKED) return p.pair ? it.qb * BLK : it.qb * ITEM_ROWS + i * BLK;
+    if constexpr (PACKED) return (it.qb * TILES + i) * p.tile_pos;
     else return it.qb * ITEM_ROWS + i * BLK;
-  };
-  auto tile_head = [&](const Item& it, int i) {
-    if constexpr (PACKED) return it.h + (p.pair ? i : 0);
-    else return it.h;
   };
   // the item that a published slot names, for the warps that read it; false: no item is left
   auto take_item = [&](int slot, int w, Item& it) {
@@ -291,7 +286,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       it.N = sched_item[8 * slot + 4];
       it.z = it.zh = 0;
       it.kh = it.h / p.group;
-      count_blocks<TILES>(it, p.causal, p.pair);
+      count_blocks<TILES>(it, p.causal, p.tile_pos);
       return w >= 0;
     } else {
       if (w >= p.total_items) return false;
@@ -388,8 +383,15 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     auto load_item = [&](const Item& it, uint32_t n) {
       mbar_wait<WAIT_PAUSE>(q_empty, (n & 1u) ^ 1u, p.status, SITE_FWD_Q);  // previous item's S MMAs are done with Q
       for (int i = 0; i < TILES; ++i) {
-        mbar_expect_tx(&q_full[i], TILE);
-        load_tile<D, FP8>(sq + i * TILE, &tm_q, &q_full[i], it.row0 + tile_row0(it, i), tile_head(it, i), it.z);
+        if constexpr (PACKED) {  // the map's dimensions are {d, head, row}: boxes of 64 columns x fold heads x tile_pos rows
+          mbar_expect_tx(&q_full[i], D * 2 * p.fold * p.tile_pos);
+#pragma unroll
+          for (int b = 0; b < D / 64; ++b)
+            tma_load_4d(sq + i * TILE + b * (BLK * 128), &tm_q, &q_full[i], b * 64, it.h, it.row0 + tile_row0(it, i), 0);
+        } else {
+          mbar_expect_tx(&q_full[i], TILE);
+          load_tile<D, FP8>(sq + i * TILE, &tm_q, &q_full[i], tile_row0(it, i), it.h, it.z);
+        }
       }
       for (int j = 0; j < it.nmax; ++j) {
         for (int kv = 0; kv < 2; ++kv) {  // K_j then V_j
@@ -402,7 +404,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     };
     if constexpr (PACKED) {
       PackedWalk walk;
-      walk.init(p, ITEM_ROWS);
+      walk.init(p, TILES);
       for (uint32_t n = 0;; ++n) {
         int w = 0;
         if (lane == 0) w = atomicAdd(p.sched_counter, 1);
@@ -410,7 +412,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         const bool more = w < walk.total;
         Item it{};
         if (more) it = walk.find(p, w);
-        count_blocks<TILES>(it, p.causal, p.pair);
+        count_blocks<TILES>(it, p.causal, p.tile_pos);
         if (lane == 0) {
           const uint32_t slot = n & 1u, sph = (n >> 1) & 1u;
           mbar_wait<WAIT_PAUSE>(&sched_empty[slot], sph ^ 1u, p.status, SITE_FWD_SCHED);
@@ -623,6 +625,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const int i = warp >> 2;                 // tile
     const uint32_t quarter = warp & 3u;      // TMEM lanes [32*quarter, +32)
     const int row_in_tile = quarter * 32 + lane;
+    // packed: the row's position in the tile and its head; rows past tile_pos * fold are nobody's
+    int pos_in_tile = row_in_tile, head_in_tile = 0;
+    if constexpr (PACKED) {
+      pos_in_tile = row_in_tile / p.fold;
+      head_in_tile = row_in_tile - pos_in_tile * p.fold;
+    }
     const uint32_t lane_addr = (quarter * 32u) << 16;
     const float scale = p.scale_log2;
     const bool vec_ok = ((reinterpret_cast<uintptr_t>(p.o) & 15) == 0) && ((p.o_sn & 7) == 0) && ((p.o_sh & 7) == 0) &&
@@ -648,9 +656,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         w = __shfl_sync(0xffffffffu, w, 0);
         if (!take_item(slot, w, it)) break;
       }
-      const int row0 = tile_row0(it, i), head = tile_head(it, i);
+      const int row0 = tile_row0(it, i), head = it.h + head_in_tile;
       const int N = PACKED ? it.N : p.N;
-      const int row = row0 + row_in_tile;  // query index
+      const int row = row0 + pos_in_tile;  // query index
+      bool valid = row < N;
+      if constexpr (PACKED) valid = valid && pos_in_tile < p.tile_pos;
       const int nb = i ? it.n1 : it.n0;
       float m_ref = -INFINITY, l = 0.f;
       float m_true = -INFINITY;  // the exact running maximum (m_ref lags it by up to the rescale threshold)
@@ -703,7 +713,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
         };
         if (traced) B200_TRACE_EVENT(p.status, i, 2);
-        // mx is finite: every row sees at least one valid column in every block it visits
+        // every row sees at least one valid column in its first block, so the running maximum is finite from there on
+        // (in a later block a folded tile's first positions may see none: mx = -inf, all weights 0)
         const float m_new = fmaxf(m_ref, mx * scale);
         m_true = fmaxf(m_true, mx * scale);
         // lazy rescale of the accumulator (the ld/st below are warp collectives, so the warp
@@ -712,7 +723,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         // as the reference does: the 2-bit mantissa of P makes its rounding depend on the scale
         // (packed: the rows behind the sequence's end hold another's values; they have no vote, or that
         // sequence's values would decide when this one's weights are rounded against which reference)
-        const bool grow = (!PACKED || row < N) && (FP8 ? (m_new > m_ref) : ((m_new - m_ref) > kRescaleThreshold<BF16>));
+        const bool grow = (!PACKED || valid) && (FP8 ? (m_new > m_ref) : ((m_new - m_ref) > kRescaleThreshold<BF16>));
         if (__any_sync(0xffffffffu, grow)) {
           // every row of the warp moves its reference point to its exact running maximum (this block
           // included): the pass over O is paid for by the row that had to move, and the others start
@@ -806,11 +817,16 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       if (traced) B200_TRACE_EVENT(p.status, i, 8);
       tc_fence_after();
       const float inv_l = 1.f / l;
-      const bool valid = row < N;
       uint16_t* orow = reinterpret_cast<uint16_t*>(p.o) + (long long)it.z * p.o_sz + (long long)head * p.o_sh +
                        (long long)(it.row0 + row) * p.o_sn;
-      // packed: a box that reaches past the sequence's end would overwrite the next one
-      if (p.o_tma && (!PACKED || row0 + (int)quarter * 32 + 32 <= N)) {
+      // packed: a box that reaches past the sequence's end would overwrite the next one (the lanes' positions rise)
+      bool boxed = p.o_tma;
+      [[maybe_unused]] unsigned rows_valid = 0;
+      if constexpr (PACKED) {
+        rows_valid = __ballot_sync(0xffffffffu, valid);
+        boxed = boxed && rows_valid == 0xffffffffu;
+      }
+      if (PACKED ? rows_valid != 0 : boxed) {
         // 64 columns at a time: scaled, packed, written to this warp's swizzled staging buffer and
         // stored by TMA (full 128-byte lines; rows past N are clipped by the hardware).  A warp-wide
         // store of one row per lane touches 32 lines per instruction and made this epilogue cost
@@ -841,7 +857,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0 && warp_row0 < N) {
-            tma_store_4d(&tm_o_map, stg, 0, warp_row0, head, it.z);
+            tma_store_4d(&tm_o_map, stg, 0, warp_row0, it.h, it.z);
             tma_store_commit();
           }
         } else
@@ -863,15 +879,31 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
               wv[k] = pack2<BF16>(__uint_as_float(o[8 * ch + 2 * k]) * inv_l, __uint_as_float(o[8 * ch + 2 * k + 1]) * inv_l);
             *reinterpret_cast<uint4*>(stg + sw128_offset(lane, ch)) = make_uint4(wv[0], wv[1], wv[2], wv[3]);
           }
+          if constexpr (PACKED) {
+            if (!boxed) {
+              // rows stored one by one, eight lanes (128 bytes) to a row: what a box cannot take
+              __syncwarp();
+#pragma unroll
+              for (int r4 = 0; r4 < 32; r4 += 4) {
+                const int r = r4 + (lane >> 3);
+                uint16_t* dst = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(orow), r));
+                const uint4 x = *reinterpret_cast<const uint4*>(stg + sw128_offset(r, lane & 7));
+                if ((rows_valid >> r) & 1u) *reinterpret_cast<uint4*>(dst + c + (lane & 7) * 8) = x;
+              }
+              __syncwarp();
+              continue;
+            }
+          }
           fence_proxy_async_smem();
           __syncwarp();
           if (traced) B200_TRACE_EVENT(p.status, i, 0xC);
-          if (lane == 0 && warp_row0 < N) {
-            tma_store_4d(&tm_o_map, stg, c, it.row0 + warp_row0, head, it.z);
+          if (lane == 0 && (PACKED || warp_row0 < N)) {
+            if constexpr (PACKED) tma_store_4d(&tm_o_map, stg, c, it.h, it.row0 + row, 0);  // (lane 0's position)
+            else tma_store_4d(&tm_o_map, stg, c, warp_row0, it.h, it.z);
             tma_store_commit();
           }
         }
-      } else {
+      } else if constexpr (!PACKED) {
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t o[32];
@@ -913,7 +945,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       if (!PACKED && valid && p.row_max) p.row_max[(long long)it.zh * p.N + row] = m_true;
       if (traced) B200_TRACE_EVENT(p.status, i, 9);
     }
-    if (p.o_tma && lane == 0) tma_store_wait_read<0>();  // the staging buffer has been read: the CTA may exit, the writes land on their own
+    if ((PACKED || p.o_tma) && lane == 0) tma_store_wait_read<0>();  // the staging buffer has been read: the CTA may exit, the writes land on their own
     teardown(false);
   }
 }
