@@ -92,6 +92,8 @@ struct PackedFwdParams : FwdParams {
   int by_level;      // order of the items, see PackedWalk
   int fold;          // heads of a tile: 1, or all of a group
   int tile_pos;      // positions of a tile: 128 / fold
+  int item_pos, item_shift;    // positions of an item, and their log2 (-1: no power of two)
+  int block_items, kv_items;   // items per block of item_pos positions, and of those per k/v head
   int zero_rest;     // rows of o that belong to no sequence: 0 left as they are, 1 set to zero
 };
 
@@ -163,7 +165,6 @@ __device__ __forceinline__ Item decode_item(const FwdParams& p, int w) {
 struct PackedWalk {
   int blocks, base, count, total;  // the class: query blocks, its first ticket, sequences in it
   int at, before;                  // where the last draw's search ended: 32 sequences from `at`, `before` of the class before them
-  int rows, heads, group;          // positions of an item; items per block of positions, and of those per k/v head
   int start0, len0, blocks0;       // of sequence `lane`: most batches need no more than this one load
   bool by_level;
 
@@ -175,10 +176,13 @@ struct PackedWalk {
     if (b < 32) return blocks0;
     int start, len;
     extent(p, b, start, len);
-    return (len + rows - 1) / rows;
+    return blocks_of(p, len);
+  }
+  static __device__ __forceinline__ int blocks_of(const PackedFwdParams& p, int len) {
+    return p.item_shift >= 0 ? (len + p.item_pos - 1) >> p.item_shift : (len + p.item_pos - 1) / p.item_pos;
   }
   __device__ __forceinline__ bool in_class(int n) const { return by_level ? n >= blocks : n == blocks; }
-  __device__ __forceinline__ int tickets() const { return count * heads * (by_level ? 1 : blocks); }
+  __device__ __forceinline__ int tickets(const PackedFwdParams& p) const { return count * p.block_items * (by_level ? 1 : blocks); }
   // the class of the most blocks below `below`
   __device__ __forceinline__ void enter(const PackedFwdParams& p, int below) {
     const int lane = threadIdx.x & 31;
@@ -192,33 +196,37 @@ struct PackedWalk {
     count = blocks > 0 ? (int)__reduce_add_sync(0xffffffffu, (unsigned)c) : 0;
     at = before = 0;
   }
-  __device__ __forceinline__ void init(const PackedFwdParams& p, int tiles) {
+  __device__ __forceinline__ void init(const PackedFwdParams& p) {
     by_level = p.by_level;
-    rows = tiles * p.tile_pos;
-    heads = p.H / p.fold;
-    group = p.group / p.fold;
     start0 = len0 = 0;
     if ((int)(threadIdx.x & 31) < p.batch) extent(p, threadIdx.x & 31, start0, len0);
-    blocks0 = (len0 + rows - 1) / rows;
+    blocks0 = blocks_of(p, len0);
     int sum = 0;
     for (int b = threadIdx.x & 31; b < p.batch; b += 32) sum += seq_blocks(p, b);
-    total = (int)__reduce_add_sync(0xffffffffu, (unsigned)sum) * heads;
+    total = (int)__reduce_add_sync(0xffffffffu, (unsigned)sum) * p.block_items;
     base = 0;
     enter(p, 0x7fffffff);
   }
   __device__ __forceinline__ Item find(const PackedFwdParams& p, int w) {  // w < total
-    while (blocks > 0 && w - base >= tickets()) {
-      base += tickets();
+    while (blocks > 0 && w - base >= tickets(p)) {
+      base += tickets(p);
       enter(p, blocks);
     }
-    const int lane = threadIdx.x & 31, per_seq = heads * (by_level ? 1 : blocks), per_kv = group * (by_level ? 1 : blocks);
-    const int nth = (w - base) / per_seq;
+    const int lane = threadIdx.x & 31, per_seq = p.block_items * (by_level ? 1 : blocks);
+    const int nth = count == 1 ? 0 : (w - base) / per_seq;
     int r = (w - base) - nth * per_seq;
     Item it;
-    it.kh = r / per_kv;
-    r -= it.kh * per_kv;
-    it.qb = blocks - 1 - r / group;  // (by level r < group)
-    it.h = it.kh * p.group + r % group;  // (folded: group = 1, the first of the heads)
+    if (by_level) {
+      it.kh = r / p.kv_items;
+      it.qb = blocks - 1;
+      r -= it.kh * p.kv_items;
+    } else {
+      it.kh = r / (p.kv_items * blocks);
+      r -= it.kh * p.kv_items * blocks;
+      it.qb = blocks - 1 - r / p.kv_items;
+      r %= p.kv_items;
+    }
+    it.h = it.kh * p.group + r;  // (folded: one item per k/v head, the first of its heads)
     it.z = it.zh = 0;
     it.row0 = it.N = 0;
     for (; at < p.batch; at += 32) {
@@ -404,11 +412,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     };
     if constexpr (PACKED) {
       PackedWalk walk;
-      walk.init(p, TILES);
+      walk.init(p);
+      // the first ticket is the CTA's number, without a draw; the counter hands out those behind the grid's
+      const int grid = (int)gridDim.x;
+      int w = blockIdx.x;
       for (uint32_t n = 0;; ++n) {
-        int w = 0;
-        if (lane == 0) w = atomicAdd(p.sched_counter, 1);
-        w = __shfl_sync(0xffffffffu, w, 0);
         const bool more = w < walk.total;
         Item it{};
         if (more) it = walk.find(p, w);
@@ -422,11 +430,18 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           sched_item[8 * slot + 3] = it.row0;
           sched_item[8 * slot + 4] = it.N;
           mbar_arrive(&sched_full[slot]);
-          if (w == walk.total + (int)gridDim.x - 1) atomicExch(p.sched_counter, 0);
-          if (more) load_item(it, n);
+          if (more) {
+            load_item(it, n);
+            const int drawn = atomicAdd(p.sched_counter, 1);
+            // every CTA that had a first item draws until its ticket is past the end: the last of those draws puts
+            // the zero back for the next launch that is handed this counter
+            if (drawn == max(walk.total - grid, 0) + min(grid, walk.total) - 1) atomicExch(p.sched_counter, 0);
+            w = grid + drawn;
+          }
         }
         __syncwarp();
         if (!more) break;
+        w = __shfl_sync(0xffffffffu, w, 0);
       }
     } else if (lane == 0) {
       for (uint32_t n = 0;; ++n) {

@@ -64,6 +64,10 @@ int launch_attn_varlen(DeviceCtx* ctx, cudaStream_t stream, const AttnVarlenArgs
   p.group = group;
   p.fold = fold;
   p.tile_pos = tile_pos;
+  p.item_pos = (a.D == 256 ? 1 : 2) * tile_pos;
+  p.item_shift = (p.item_pos & (p.item_pos - 1)) == 0 ? __builtin_ctz((unsigned)p.item_pos) : -1;
+  p.block_items = a.Hq / fold;
+  p.kv_items = group / fold;
   // By level evens out the end of a causal launch (2 to 8 % over by length: 16 x 2048 rows at 16/1 heads 291 against
   // 308 us, 2000 rows at 32/8 heads 39 against 52), but comes back to every K and V once per level: with a k/v
   // head per query head and more K and V than L2 keeps that costs more (4 x 4096 at 32/32 heads 569 against
@@ -74,8 +78,7 @@ int launch_attn_varlen(DeviceCtx* ctx, cudaStream_t stream, const AttnVarlenArgs
   p.status = ctx->status;
   p.sched_counter = next_sched_counter(ctx, stream);
   if (!p.sched_counter) return B200_ERR_CUDA;
-  const int item_pos = (a.D == 256 ? 1 : 2) * tile_pos;
-  const long long most_items = ((long long)a.T / item_pos + a.batch) * (a.Hq / fold);  // the lengths are on the device
+  const long long most_items = ((long long)a.T / p.item_pos + a.batch) * p.block_items;  // the lengths are on the device
   const bool bf16 = a.dtype == B200_BF16;
   if (a.D == 256) return bf16 ? launch_packed_t<256, true>(ctx, stream, tq, tk, tv, to, p, most_items) : launch_packed_t<256, false>(ctx, stream, tq, tk, tv, to, p, most_items);
   if (a.D == 128) return bf16 ? launch_packed_t<128, true>(ctx, stream, tq, tk, tv, to, p, most_items) : launch_packed_t<128, false>(ctx, stream, tq, tk, tv, to, p, most_items);
