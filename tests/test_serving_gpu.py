@@ -784,3 +784,39 @@ def test_varlen_short_sequences_all_heads_of_a_group_to_a_tile(hq, hkv, D, causa
     v[off[-1]:] = math.nan
     again = tb.attention_varlen(q, k, v, cu, causal, 0.1)
     assert torch.equal(again[:off[4]], o[:off[4]]) and torch.equal(again[off[5]:], o[off[5]:])
+
+
+def test_calls_on_several_streams_at_once():
+    """Eager packed calls on two streams and a replayed graph on a third, over and over: each gives its own result."""
+    packs = [pack([900, 40, 333], 8, 2, 64, torch.float16, seed=101), pack([5] * 50, 4, 4, 64, torch.bfloat16, seed=102),
+             pack([2000], 4, 1, 128, torch.float16, seed=103)]
+    want = [tb.attention_varlen(q, k, v, cu, True, 0.1) for q, k, v, cu, _ in packs]
+    streams = [torch.cuda.Stream() for _ in packs]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=streams[2]):
+        q, k, v, cu, _ = packs[2]
+        captured = tb.attention_varlen(q, k, v, cu, True, 0.1)
+    for _ in range(20):
+        got = []
+        for (q, k, v, cu, _), st in zip(packs[:2], streams):
+            with torch.cuda.stream(st):
+                got.append(tb.attention_varlen(q, k, v, cu, True, 0.1))
+        with torch.cuda.stream(streams[2]):
+            captured.zero_()
+            graph.replay()
+        torch.cuda.synchronize()
+        for g, w in zip(got + [captured], want):
+            assert torch.equal(g, w)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_decode_every_length_around_the_chunks_and_slabs(D):
+    """Lengths on and beside multiples of 16 and of the chunks, under tables that make one chunk, a cluster, a join."""
+    for width, batch in ((8, 40), (64, 12), (700, 9)):
+        lens = [max(0, width * 16 - d) for d in range(batch)]
+        lens[-1] = 16 * (width // 2) + 1
+        c, table = filled_cache(lens, 1, 16, D, seed=width + D)
+        q = torch.randn(batch, 3, D, device=DEV, generator=torch.Generator(device=DEV).manual_seed(width)).bfloat16()
+        o, M = c.attend(q, table, torch.tensor(lens, dtype=I32, device=DEV), 0.11, return_stats=True)
+        check_decode(o, M, q, c, table, lens, 0.11, f"width {width}")
