@@ -820,3 +820,16 @@ def test_decode_every_length_around_the_chunks_and_slabs(D):
         q = torch.randn(batch, 3, D, device=DEV, generator=torch.Generator(device=DEV).manual_seed(width)).bfloat16()
         o, M = c.attend(q, table, torch.tensor(lens, dtype=I32, device=DEV), 0.11, return_stats=True)
         check_decode(o, M, q, c, table, lens, 0.11, f"width {width}")
+
+
+def test_varlen_refuses_an_unaligned_out():
+    q, k, v, cu, _ = pack([10], 2, 1, 64, torch.float16, seed=111)
+    odd = torch.zeros(10 * 2 * 64 + 8, dtype=torch.float16, device=DEV)
+    wide = torch.zeros(10, 2, 68, dtype=torch.float16, device=DEV)
+    for out in (odd[1:1281].view(10, 2, 64), wide[..., :64]):
+        with pytest.raises(RuntimeError, match="aligned|multiple"):
+            tb.attention_varlen(q, k, v, cu, True, 0.1, out=out)
+    big = pack([3000], 4, 1, 64, torch.float16, seed=112)  # through boxes
+    with pytest.raises(RuntimeError, match="aligned|multiple"):
+        tb.attention_varlen(*big[:4], True, 0.1, out=torch.zeros(3000, 4, 68, dtype=torch.float16, device=DEV)[..., :64])
+    assert (odd == 0).all() and (wide == 0).all()
