@@ -833,3 +833,29 @@ def test_varlen_refuses_an_unaligned_out():
     with pytest.raises(RuntimeError, match="aligned|multiple"):
         tb.attention_varlen(*big[:4], True, 0.1, out=torch.zeros(3000, 4, 68, dtype=torch.float16, device=DEV)[..., :64])
     assert (odd == 0).all() and (wide == 0).all()
+
+
+# ------------------------------------------------------------------ values that are not finite, and masked places
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("hq,hkv,D", [(2, 2, 64), (2, 2, 128), (4, 2, 128), (2, 2, 256)])
+def test_varlen_bad_keys_at_every_column(hq, hkv, D, bad, causal):
+    """A key of NaN, or one whose score is +inf, at every position mod 16 of the first and the second block: every
+    row that sees it is NaN, and only those."""
+    n, group = 160, hq // hkv
+    q, k, v, cu, off = pack([n] * 32, hq, hkv, D, torch.bfloat16, seed=121 + D)
+    q[..., 0] = 1.0
+    clean = k.clone()
+    at = [b % 16 + 16 + (112 if b >= 16 else 0) for b in range(32)]
+    for b in range(32):
+        k[off[b] + at[b], :, 0] = bad
+    o, M = tb.attention_varlen(q, k, v, cu, causal, 0.1, return_stats=True)
+    dense = lambda t: t.view(32, n, -1, D).transpose(1, 2).repeat_interleave(hq // t.shape[1], 1).contiguous()
+    o2, M2 = tb.attention_forward(dense(q), dense(k), dense(v), causal, 0.1)  # the dense form of the kernel
+    o2, M2 = o2.transpose(1, 2).reshape(o.shape), M2.transpose(0, 1).reshape(M.shape)
+    assert torch.equal(torch.isnan(o2), torch.isnan(o)) and torch.equal(torch.isnan(M2), torch.isnan(M))
+    for b in range(32):
+        first = off[b] + at[b] if causal else off[b]
+        assert torch.isnan(o[first:off[b + 1]]).all(), f"a key at position {at[b]} is not seen"
+        assert torch.isnan(M[:, first:off[b + 1]]).all()
+        check_pack(o[off[b]:first], None, q[off[b]:first], clean[off[b]:first], v[off[b]:first], [0, first - off[b]], True, 0.1)

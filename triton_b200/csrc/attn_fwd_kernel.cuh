@@ -257,6 +257,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   constexpr int ITEM_ROWS = TILES * BLK;
   constexpr int MMA_WARP = 8, TMA_WARP = 9;
   constexpr bool WAIT_PAUSE = (D != 64);  // see mbar_wait_slow
+  // The running maximum is NaN once a score was, where some weights come from the cubic.  (Head dim 64 and the 8-bit
+  // forward have them all from ex2, which passes a NaN on; at head dim 64 the 1 to 2 % that this costs buy nothing.)
+  constexpr bool KEEP_NAN = !FP8 && D != 64;
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t pad = (1024u - (smem_u32(smem_raw) & 1023u)) & 1023u;
@@ -707,12 +710,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
 #pragma unroll
           for (int u = 0; u < 16; ++u)  // three-input maximum: one instruction per column pair
-            mx4[u] = max3(mx4[u], __uint_as_float(r[c + 2 * u]), __uint_as_float(r[c + 2 * u + 1]));
+            mx4[u] = max3<KEEP_NAN>(mx4[u], __uint_as_float(r[c + 2 * u]), __uint_as_float(r[c + 2 * u + 1]));
           if (c + 32 < BLK) tmem_ld_wait32(r + c + 32);
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) mx4[u] = fmaxf(max3(mx4[u], mx4[u + 4], mx4[u + 8]), mx4[u + 12]);
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+        for (int u = 0; u < 4; ++u) mx4[u] = max2<KEEP_NAN>(max3<KEEP_NAN>(mx4[u], mx4[u + 4], mx4[u + 8]), mx4[u + 12]);
+        const float mx = max2<KEEP_NAN>(max2<KEEP_NAN>(mx4[0], mx4[1]), max2<KEEP_NAN>(mx4[2], mx4[3]));
         if constexpr (SEP_P) {
           // S_i(j) is in registers: the S buffer may take S_i(j+1)
           tc_fence_before();
@@ -731,14 +734,14 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         // every row sees at least one valid column in its first block, so the running maximum is finite from there on
         // (in a later block a folded tile's first positions may see none: mx = -inf, all weights 0)
         const float m_new = fmaxf(m_ref, mx * scale);
-        m_true = fmaxf(m_true, mx * scale);
+        m_true = max2<KEEP_NAN>(m_true, mx * scale);
         // lazy rescale of the accumulator (the ld/st below are warp collectives, so the warp
         // rescales if any of its rows has to)
         // true on the first block (m_ref = -inf).  The 8-bit forward follows the exact running maximum,
         // as the reference does: the 2-bit mantissa of P makes its rounding depend on the scale
         // (packed: the rows behind the sequence's end hold another's values; they have no vote, or that
         // sequence's values would decide when this one's weights are rounded against which reference)
-        const bool grow = (!PACKED || valid) && (FP8 ? (m_new > m_ref) : ((m_new - m_ref) > kRescaleThreshold<BF16>));
+        const bool grow = (!PACKED || valid) && (FP8 ? (m_new > m_ref) : (((KEEP_NAN ? m_true : m_new) - m_ref) > kRescaleThreshold<BF16>));
         if (__any_sync(0xffffffffu, grow)) {
           // every row of the warp moves its reference point to its exact running maximum (this block
           // included): the pass over O is paid for by the row that had to move, and the others start
@@ -762,7 +765,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         }
         if (traced) B200_TRACE_EVENT(p.status, i, 3);
         wait_pv();  // (head dim 64) before the exponential loop, not inside it: a wait in the unrolled loop keeps the compiler from interleaving its chunks
-        const float neg_m = -m_ref;
+        // a row that has seen a NaN or +inf: NaN, which makes all its weights NaN (without it the cubic below, which
+        // knows neither, would give such a key a finite weight at some positions)
+        const float neg_m = KEEP_NAN ? fmaf(m_true, 0.f, -m_ref) : -m_ref;
         float sum4[4] = {0.f, 0.f, 0.f, 0.f};
         [[maybe_unused]] uint64_t sum2[2] = {pk2(0.f, 0.f), pk2(0.f, 0.f)};
         [[maybe_unused]] const uint64_t scale2 = pk2(scale, scale), neg_m2 = pk2(neg_m, neg_m);

@@ -511,11 +511,23 @@ __device__ __forceinline__ uint32_t pack4_e5m2(float a, float b, float c, float 
   const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E5M2);
   return lo | (hi << 16);
 }
-// three-input maximum (one instruction on sm_100)
+// three-input maximum (one instruction on sm_100); KEEP_NAN: of operands with a NaN it is NaN, not the largest other
+template <bool KEEP_NAN = false>
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  if constexpr (KEEP_NAN) asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  else asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+}
+template <bool KEEP_NAN = false>
+__device__ __forceinline__ float max2(float a, float b) {
+  if constexpr (KEEP_NAN) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+  } else {
+    return fmaxf(a, b);
+  }
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -552,9 +564,9 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
-// 2^x for a pair of values in (-inf, 9] without the special-function unit: x = n + f with n = floor(x)
+// 2^x for a pair of values up to 126 without the special-function unit: x = n + f with n = floor(x)
 // (the low mantissa bits of x + 1.5 * 2^23 rounded down), 2^f by a cubic with 8.6e-5 relative error
-// (below the rounding of the 16-bit P it feeds), n added to the exponent field.
+// (below the rounding of the 16-bit P it feeds), n added to the exponent field.  Not for NaN or +inf.
 __device__ __forceinline__ void ex2_cubic2(float x0, float x1, float& p0, float& p1) {
   const uint64_t x = pk2(fmaxf(x0, -125.f), fmaxf(x1, -125.f));
   const uint64_t magic = pk2(12582912.f, 12582912.f);
