@@ -859,3 +859,17 @@ def test_varlen_bad_keys_at_every_column(hq, hkv, D, bad, causal):
         assert torch.isnan(o[first:off[b + 1]]).all(), f"a key at position {at[b]} is not seen"
         assert torch.isnan(M[:, first:off[b + 1]]).all()
         check_pack(o[off[b]:first], None, q[off[b]:first], clean[off[b]:first], v[off[b]:first], [0, first - off[b]], True, 0.1)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_masked_weights_are_zero(D):
+    """Values near bf16's largest behind a row, where causal masking hides them, add nothing to it."""
+    q, k, v, cu, off = pack([100, 300], 2, 2, D, torch.bfloat16, seed=131)
+    v[50:100] = 1e38
+    v[300:] = 1e38
+    o = tb.attention_varlen(q, k, v, cu, True, 0.1)
+    check_pack(o[:50], None, q[:50], k[:50], v[:50], [0, 50], True, 0.1)
+    check_pack(o[100:300], None, q[100:300], k[100:300], v[100:300], [0, 200], True, 0.1)
+    dense = lambda t: t[100:].transpose(0, 1)[None].contiguous()
+    o, _ = tb.attention_forward(dense(q), dense(k), dense(v), True, 0.1)
+    check_pack(o[0, :, :200].transpose(0, 1), None, q[100:300], k[100:300], v[100:300], [0, 200], True, 0.1)

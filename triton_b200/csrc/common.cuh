@@ -567,8 +567,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // 2^x for a pair of values up to 126 without the special-function unit: x = n + f with n = floor(x)
 // (the low mantissa bits of x + 1.5 * 2^23 rounded down), 2^f by a cubic with 8.6e-5 relative error
 // (below the rounding of the 16-bit P it feeds), n added to the exponent field.  Not for NaN or +inf.
+// Exactly 0 at -127 and below: there f = 0 and the cubic is 1, whose exponent field n takes to zero; what lies between
+// -127 and -126 becomes a subnormal number below 2^-126.
 __device__ __forceinline__ void ex2_cubic2(float x0, float x1, float& p0, float& p1) {
-  const uint64_t x = pk2(fmaxf(x0, -125.f), fmaxf(x1, -125.f));
+  const uint64_t x = pk2(fmaxf(x0, -127.f), fmaxf(x1, -127.f));
   const uint64_t magic = pk2(12582912.f, 12582912.f);
   uint64_t t;
   asm("add.rm.f32x2 %0, %1, %2;" : "=l"(t) : "l"(x), "l"(magic));
