@@ -873,3 +873,22 @@ def test_masked_weights_are_zero(D):
     dense = lambda t: t[100:].transpose(0, 1)[None].contiguous()
     o, _ = tb.attention_forward(dense(q), dense(k), dense(v), True, 0.1)
     check_pack(o[0, :, :200].transpose(0, 1), None, q[100:300], k[100:300], v[100:300], [0, 200], True, 0.1)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_varlen_a_first_block_of_minus_infinity(D, dtype):
+    """Scores of -inf have weight 0, also where a whole block of keys has nothing else."""
+    q, k, v, cu, off = pack([400], 2, 1, D, dtype, seed=141)
+    q = q.abs() + 0.1
+    k[:128] = -math.inf
+    o, M = tb.attention_varlen(q, k, v, cu, False, 0.1, return_stats=True)
+    for h in range(2):
+        want = one_head(q[:, h], k[128:, 0], v[128:, 0], 0.1, False)
+        check(o[:, h], want, dtype, dtype, f"head {h}")
+        check_lse(M[h], want, f"lse of head {h}")
+    o = tb.attention_varlen(q, k, v, cu, True, 0.1)
+    assert torch.isnan(o[:128]).all()  # nothing but -inf: 0 / 0
+    for h in range(2):
+        want = one_head(q[128:, h], k[128:, 0], v[128:, 0], 0.1, True)
+        check(o[128:, h], want, dtype, dtype, f"causal, head {h}")

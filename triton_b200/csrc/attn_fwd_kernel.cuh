@@ -40,6 +40,7 @@
 // at head dim 128, and columns [320,384) / [448,512) at head dim 64 (16-bit), where S_i of the next
 // block is then issued before P_i V of this one.  Head dim 256: S [0,128), O [256,512).
 #pragma once
+#include <cfloat>
 #include <cmath>
 #include <cstdlib>
 #include <type_traits>
@@ -731,22 +732,23 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           }
         };
         if (traced) B200_TRACE_EVENT(p.status, i, 2);
-        // every row sees at least one valid column in its first block, so the running maximum is finite from there on
-        // (in a later block a folded tile's first positions may see none: mx = -inf, all weights 0)
+        // (mx = -inf: all scores of the block are, or a folded tile's first positions see none of a later block; weights 0)
         const float m_new = fmaxf(m_ref, mx * scale);
         m_true = max2<KEEP_NAN>(m_true, mx * scale);
         // lazy rescale of the accumulator (the ld/st below are warp collectives, so the warp
         // rescales if any of its rows has to)
-        // true on the first block (m_ref = -inf).  The 8-bit forward follows the exact running maximum,
+        // true on the first block (m_ref = -inf), also if all its scores are -inf and the difference is NaN.  The 8-bit forward follows the exact running maximum,
         // as the reference does: the 2-bit mantissa of P makes its rounding depend on the scale
         // (packed: the rows behind the sequence's end hold another's values; they have no vote, or that
         // sequence's values would decide when this one's weights are rounded against which reference)
-        const bool grow = (!PACKED || valid) && (FP8 ? (m_new > m_ref) : (((KEEP_NAN ? m_true : m_new) - m_ref) > kRescaleThreshold<BF16>));
+        const bool grow = (!PACKED || valid) && (FP8 ? (m_new > m_ref) : !((m_new - m_ref) <= kRescaleThreshold<BF16>));
         if (__any_sync(0xffffffffu, grow)) {
           // every row of the warp moves its reference point to its exact running maximum (this block
           // included): the pass over O is paid for by the row that had to move, and the others start
           // their next window from zero lag.  (Leaving 6 log2 units of headroom above the maximum as
           // well bought another 2-3 % on sharply peaked scores; not taken: it costs P 6 bits of range.)
+          // (finite where the scores so far are all -inf: against it they have weight 0 and not NaN)
+          if (!FP8) m_true = max2<KEEP_NAN>(m_true, -FLT_MAX);
           const float m_to = FP8 ? m_new : m_true;
           const float alpha = (FP8 && !grow) ? 1.f : ex2(m_ref - m_to);  // 0 on the first block
           if (!FP8 || grow) { m_ref = m_to; l *= alpha; }
@@ -962,7 +964,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       } else if (valid) {
         p.m[(long long)it.zh * p.N + row] = m_ref + log2f(l);
       }
-      if (!PACKED && valid && p.row_max) p.row_max[(long long)it.zh * p.N + row] = m_true;
+      if (!PACKED && valid && p.row_max) p.row_max[(long long)it.zh * p.N + row] = m_true == -FLT_MAX ? -INFINITY : m_true;
       if (traced) B200_TRACE_EVENT(p.status, i, 9);
     }
     if ((PACKED || p.o_tma) && lane == 0) tma_store_wait_read<0>();  // the staging buffer has been read: the CTA may exit, the writes land on their own
