@@ -892,3 +892,18 @@ def test_varlen_a_first_block_of_minus_infinity(D, dtype):
     for h in range(2):
         want = one_head(q[128:, h], k[128:, 0], v[128:, 0], 0.1, True)
         check(o[128:, h], want, dtype, dtype, f"causal, head {h}")
+
+
+def test_varlen_statistics_of_rows_outside_the_sequences_with_out():
+    """M is the call's own tensor: -inf for rows that belong to no sequence, whether O is or not."""
+    for D in (64, 32):
+        q, k, v, cu, off = pack([130, 9], 2, 2, D, torch.float16, seed=151, tail=150)
+        for offsets, inside in ((cu, slice(0, 139)), (cu + 20, slice(20, 159)), (ints(0), slice(0, 0))):
+            before = torch.full((2, 289), 5.0, device=DEV)  # what the allocator hands out next
+            del before
+            mine = torch.full_like(q, 7.0)
+            o, M = tb.attention_varlen(q, k, v, offsets, True, 0.2, out=mine, return_stats=True)
+            rest = torch.ones(289, dtype=torch.bool, device=DEV)
+            rest[inside] = False
+            assert (M[:, rest] == -math.inf).all() and torch.isfinite(M[:, inside]).all()
+            assert (mine[rest] == 7.0).all()

@@ -95,7 +95,7 @@ struct PackedFwdParams : FwdParams {
   int tile_pos;      // positions of a tile: 128 / fold
   int item_pos, item_shift;    // positions of an item, and their log2 (-1: no power of two)
   int block_items, kv_items;   // items per block of item_pos positions, and of those per k/v head
-  int zero_rest;     // rows of o that belong to no sequence: 0 left as they are, 1 set to zero
+  int rest;          // rows that belong to no sequence: bit 0 set to zero in o, bit 1 set to -inf in m
 };
 
 // FP8: Q, K, V, P and O are 8-bit (e5m2, the reference's fp8 forward, 06-fused-attention.py:38-40,
@@ -368,15 +368,15 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     // nothing else: these warps only lend registers and take part in the barriers at both ends
     // (at head dim 256 the second tile's softmax warpgroup has no tile)
     if constexpr (PACKED) {
-      if (p.zero_rest && warp >= 12) {
+      if (p.rest && warp >= 12) {
         const int first = min(max(p.cu[0], 0), p.N), end = max(min(p.cu[p.batch], p.N), first);
         const long long per_row = (long long)p.H * (D / 8);
         for (long long at = (long long)blockIdx.x * 128 + (threadIdx.x - 384); at < (first + p.N - end) * per_row;
              at += (long long)gridDim.x * 128) {
           const long long r = at / per_row, row = r < first ? r : r - first + end;
           const int h = (int)(at % per_row) / (D / 8), d = (int)(at % (D / 8)) * 8;
-          *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.o) + row * p.o_sn + h * p.o_sh + d) = make_uint4(0u, 0u, 0u, 0u);
-          if (d == 0 && p.m) p.m[(long long)h * p.N + row] = -INFINITY;
+          if (p.rest & 1) *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.o) + row * p.o_sn + h * p.o_sh + d) = make_uint4(0u, 0u, 0u, 0u);
+          if (d == 0 && (p.rest & 2)) p.m[(long long)h * p.N + row] = -INFINITY;
         }
       }
     }

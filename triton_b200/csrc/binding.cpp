@@ -100,7 +100,7 @@ py::object attention_varlen(const Tensor& q, const Tensor& k, const Tensor& v, c
   check(varlen_fwd(stream_of(dev), q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.mutable_data_ptr(),
                    stats ? m.mutable_data_ptr<float>() : nullptr, cu.const_data_ptr<int>(), small(cu.size(0) - 1), small(T),
                    small(Hq), small(Hkv), small(D), q.strides().data(), k.strides().data(), v.strides().data(),
-                   o.strides().data(), static_cast<float>(sm_scale), causal, dtype_of(q), !out),
+                   o.strides().data(), static_cast<float>(sm_scale), causal, dtype_of(q), out ? 2 : 1),
         "attention_varlen");
   return result(o, m, stats);
 }

@@ -638,13 +638,14 @@ int b200_attention_varlen_fwd(b200_stream_t stream, const void* q, const void* k
   if (((long long)T / 128 + batch + 1) * Hq > 0x3fffffffLL) return fail(B200_ERR_UNSUPPORTED, "too many work items");
   DeviceCtx* ctx = ready_ctx();
   if (!ctx) return g_err_code;
-  if (T == 0 || Hq == 0 || (batch == 0 && !zero_rest)) return B200_OK;
+  const int rest = (zero_rest && zero_rest != 2 ? 1 : 0) | (zero_rest && m ? 2 : 0);
+  if (T == 0 || Hq == 0 || (batch == 0 && !rest)) return B200_OK;
   if (!q || !k || !v || !o || !cu_seqlens) return fail(B200_ERR_ARG, "null pointer");
   AttnVarlenArgs a{};
   a.q = q; a.k = k; a.v = v; a.o = o; a.m = m; a.cu = cu_seqlens;
   a.batch = batch; a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.D = D;
   for (int i = 0; i < 2; ++i) { a.sq[i] = stride_q[i]; a.sk[i] = stride_k[i]; a.sv[i] = stride_v[i]; a.so[i] = stride_o[i]; }
-  a.sm_scale = sm_scale; a.causal = causal ? 1 : 0; a.dtype = dtype; a.zero_rest = zero_rest ? 1 : 0;
+  a.sm_scale = sm_scale; a.causal = causal ? 1 : 0; a.dtype = dtype; a.rest = rest;
   return launch_attn_varlen(ctx, reinterpret_cast<cudaStream_t>(stream), a);
 }
 

@@ -54,7 +54,8 @@ struct AttnVarlenArgs {
   int batch, T, Hq, Hkv, D;
   long long sq[2], sk[2], sv[2], so[2];
   float sm_scale;
-  int causal, dtype, zero_rest;
+  int causal, dtype;
+  int rest;  // see PackedFwdParams
 };
 int launch_attn_varlen(DeviceCtx* ctx, cudaStream_t stream, const AttnVarlenArgs& a);
 

@@ -28,8 +28,8 @@ def attention_varlen(q, k, v, cu_seqlens, causal, sm_scale, *, out=None, return_
     directions.  Head dims 16 .. 256 as in attention().  Any strides with a contiguous head dimension and the
     others multiples of 8 (slices of one fused projection, say).  Returns O [T, Hq, D], with
     return_stats=True (O, M): M [Hq, T] is the base-2 log-sum-exp of attention_forward.
-    Rows of T that belong to no sequence (padding behind the last one) come back as zeros (-inf in M); with
-    `out=` they stay as they were.
+    Rows of T that belong to no sequence (padding behind the last one) come back as zeros, with `out=` they stay
+    as they were; in M they are -inf.
     """
     if q.dim() == 3 and q.shape[2] in (16, 32):  # as in attention_forward: zero-padded to the kernels' head dim 64
         D = q.shape[2]
