@@ -124,3 +124,8 @@ def test_custom_ops_trace_on_meta_tensors():
     assert ns.kv_cache_append(*c, k, k, table, lens) is None
     o = ns.attention_decode(q, *c, table, lens, 0.5)
     assert o.shape == q.shape and o.dtype == q.dtype
+
+
+def test_docstrings_end_where_their_sentences_do():
+    for f in (tb.attention_varlen, tb.kv_cache_append, tb.attention_decode, tb.PagedKVCache):
+        assert f.__doc__.rstrip().endswith("."), f.__name__

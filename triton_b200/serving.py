@@ -52,7 +52,7 @@ def kv_cache_append(k_cache, v_cache, k_scale, v_scale, k, v, page_table, seq_le
     row per sequence without cu_seqlens (T == batch).
     The scale of a page and head is a power of two, 2^e with the smallest e >= -126 that lets e4m3's 448 * 2^e
     reach every finite value; values are stored as x / scale rounded to nearest even, non-finite ones as NaN.
-  XX    """
+    """
     (_lib._binding or _lib.binding()).kv_cache_append(k_cache, v_cache, k_scale, v_scale, k, v, page_table, seq_lens, cu_seqlens)
 
 
