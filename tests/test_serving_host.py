@@ -129,3 +129,21 @@ def test_custom_ops_trace_on_meta_tensors():
 def test_docstrings_end_where_their_sentences_do():
     for f in (tb.attention_varlen, tb.kv_cache_append, tb.attention_decode, tb.PagedKVCache):
         assert f.__doc__.rstrip().endswith("."), f.__name__
+
+
+def test_dual_tensors_are_refused():
+    """A dual tensor of forward-mode differentiation does not pass a call in silence, neither while autograd records nor
+    under no_grad."""
+    from torch.autograd import forward_ad
+    q, k, v, cu = _pack()
+    c, table, lens = _cache()
+    q1 = torch.zeros(3, 4, 64, dtype=torch.float16)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        calls = [lambda: tb.attention_varlen(dual(q), k, v, cu, True, 0.5), lambda: tb.attention_varlen(q, k, dual(v), cu, True, 0.5),
+                 lambda: tb.kv_cache_append(*c, dual(q1[:, :2]), q1[:, :2], table, lens), lambda: tb.attention_decode(dual(q1), *c, table, lens, 0.5)]
+        for call in calls:
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no forward-mode derivative"):  # which ends backward recording only
+                call()

@@ -45,6 +45,10 @@ void check(int code, const char* what) {
   if (code) refuse(std::string("triton_b200 error [") + what + "] code " + std::to_string(code) + ": " + last_error());
 }
 void no_grad(const char* what, std::initializer_list<const Tensor*> ts) {
+  // (torch.no_grad ends the recording of backward passes only: a dual tensor keeps its tangent under it)
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    for (const Tensor* t : ts)
+      if (t->_fw_grad(0).defined()) refuse(std::string(what) + " has no forward-mode derivative");
   if (!at::GradMode::is_enabled()) return;
   for (const Tensor* t : ts)
     if (t->requires_grad())

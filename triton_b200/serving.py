@@ -7,7 +7,8 @@
 
 The reference's attention takes dense batches of one length and one head count
 (python/tutorials/06-fused-attention.py:441-475); these three are what a program that answers needs beside
-it.  They are for inference: inputs that require a gradient are refused while autograd records.
+it.  They are for inference: inputs that require a gradient are refused while autograd records, dual tensors of
+forward-mode differentiation always.
 
 All lengths, offsets and page tables are int32 CUDA tensors that the kernels read: no call synchronises, and
 every call can be captured into a CUDA graph (whose replays see the tensors' current values).
