@@ -147,3 +147,19 @@ def test_dual_tensors_are_refused():
                 call()
             with torch.no_grad(), pytest.raises(RuntimeError, match="no forward-mode derivative"):  # which ends backward recording only
                 call()
+
+
+def test_a_cache_that_requires_a_gradient_is_refused():
+    from torch.autograd import forward_ad
+    c, table, lens = _cache()
+    q = torch.zeros(3, 4, 64, dtype=torch.float16)
+    for i in range(4):
+        d = [x.clone().requires_grad_(True) if j == i else x for j, x in enumerate(c)]
+        with pytest.raises(RuntimeError, match="no backward"):
+            tb.attention_decode(q, *d, table, lens, 0.5)
+        with pytest.raises(RuntimeError, match="no backward"):
+            tb.kv_cache_append(*d, q[:, :2], q[:, :2], table, lens)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU fallback"):
+            tb.attention_decode(q, *d, table, lens, 0.5)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+        tb.attention_decode(q, *c[:3], forward_ad.make_dual(c[3], torch.ones_like(c[3])), table, lens, 0.5)

@@ -139,7 +139,7 @@ void kv_cache_append(const Tensor& k_cache, const Tensor& v_cache, const Tensor&
   require(half_type(k) && v.scalar_type() == k.scalar_type(), "fp16 or bf16, one type");
   if (cu) ints(*cu, batch + 1, "cu_seqlens must be a contiguous int32 tensor [batch + 1]");
   else require(k.size(0) == batch, "without cu_seqlens every sequence has one new row");
-  no_grad("kv_cache_append", {&k, &v});
+  no_grad("kv_cache_append", {&k, &v, &k_cache, &v_cache, &k_scale, &v_scale});
   const c10::Device dev = one_device({&k_cache, &v_cache, &k_scale, &v_scale, &k, &v, &table, &lens});
   if (cu) one_device({&k, &*cu});
   c10::cuda::CUDAGuard guard(dev);
@@ -160,7 +160,7 @@ py::object attention_decode(const Tensor& q, const Tensor& k_cache, const Tensor
   const int Hq = small(q.size(1));
   require(c.heads > 0 && Hq % c.heads == 0, "the query heads must be a multiple of the cache's heads");
   require(half_type(q), "fp16 or bf16");
-  no_grad("attention_decode", {&q});
+  no_grad("attention_decode", {&q, &k_cache, &v_cache, &k_scale, &v_scale});
   const c10::Device dev = one_device({&q, &k_cache, &v_cache, &k_scale, &v_scale, &table, &lens});
   c10::cuda::CUDAGuard guard(dev);
   const Tensor o = output(out, q, dev);
