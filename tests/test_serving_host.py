@@ -163,3 +163,28 @@ def test_a_cache_that_requires_a_gradient_is_refused():
             tb.attention_decode(q, *d, table, lens, 0.5)
     with forward_ad.dual_level(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
         tb.attention_decode(q, *c[:3], forward_ad.make_dual(c[3], torch.ones_like(c[3])), table, lens, 0.5)
+
+
+def test_binding_is_rebuilt_for_another_torch(tmp_path, monkeypatch):
+    """The binding is linked against torch's libraries: built for another version of it, it is stale."""
+    from triton_b200 import build
+    made = []
+
+    class Done:
+        returncode, stdout, stderr = 0, "", ""
+
+    def compiler(cmd, **kw):
+        made.append(cmd)
+        open(build.BINDING, "w").close()
+        return Done
+
+    monkeypatch.setattr(build, "BINDING", str(tmp_path / "_binding.so"))
+    monkeypatch.setattr(build, "OBJ", str(tmp_path / "_obj"))
+    monkeypatch.setattr(build.subprocess, "run", compiler)
+    build.build_binding()
+    build.build_binding()
+    assert len(made) == 1
+    monkeypatch.setattr(torch, "__version__", torch.__version__ + "+other")
+    build.build_binding()
+    build.build_binding()
+    assert len(made) == 2

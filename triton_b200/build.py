@@ -47,10 +47,13 @@ def _newest_header():
 def build_binding(force=False, verbose=False):
     src = os.path.join(CSRC, "binding.cpp")
     newest = max(os.path.getmtime(src), os.path.getmtime(os.path.join(ROOT, "include", "triton_b200.h")))
-    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= newest:
-        return BINDING
     import sysconfig
     import torch
+    # what it was built against, beside the objects: another torch or Python makes it stale whatever its time
+    against, stamp = f"torch {torch.__version__} at {torch.__file__}, {sys.implementation.cache_tag}\n", os.path.join(OBJ, "binding.txt")
+    fresh = os.path.exists(BINDING) and os.path.getmtime(BINDING) >= newest and os.path.exists(stamp)
+    if not force and fresh and open(stamp).read() == against:
+        return BINDING
     home = os.path.dirname(os.path.abspath(torch.__file__))
     inc = os.path.join(home, "include")
     cuda = os.path.dirname(os.path.dirname(os.path.realpath(_nvcc())))
@@ -64,6 +67,9 @@ def build_binding(force=False, verbose=False):
         sys.stderr.write(" ".join(cmd) + "\n" + r.stdout + r.stderr)
     if r.returncode != 0:
         raise RuntimeError("the compiler failed for binding.cpp")
+    os.makedirs(OBJ, exist_ok=True)
+    with open(stamp, "w") as f:
+        f.write(against)
     return BINDING
 
 
