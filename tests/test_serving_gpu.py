@@ -907,3 +907,27 @@ def test_varlen_statistics_of_rows_outside_the_sequences_with_out():
             rest[inside] = False
             assert (M[:, rest] == -math.inf).all() and torch.isfinite(M[:, inside]).all()
             assert (mine[rest] == 7.0).all()
+
+
+def test_decode_large_queries_over_small_keys():
+    """q near the end of bf16's range, keys at the other: the score is an ordinary number and so is the output."""
+    lens = [200]
+    c, table = filled_cache(lens, 1, 32, 64, seed=161)
+    g = torch.Generator(device=DEV).manual_seed(7)
+    q = ((1 + torch.rand(1, 4, 64, device=DEV, generator=g)) * torch.randn(1, 4, 64, device=DEV, generator=g).sign()).bfloat16()
+    o0, M0 = c.attend(q, table, ints(200), 8.0, return_stats=True)
+    check_decode(o0, M0, q, c, table, lens, 8.0)
+    k_scale = c.k_scale.clone()  # 2^-8 .. 2^-3
+    for e in (100, 117):
+        c.k_scale.copy_(k_scale * 2.0 ** -e)
+        o, M = c.attend((q.double() * 2.0 ** e).bfloat16(), table, ints(200), 8.0, return_stats=True)
+        assert torch.equal(o, o0) and torch.equal(M, M0)
+        if e == 100:
+            c.k_scale.copy_(k_scale * 2.0 ** e)
+            o, M = c.attend((q.double() * 2.0 ** -e).bfloat16(), table, ints(200), 8.0, return_stats=True)
+            assert torch.equal(o, o0) and torch.equal(M, M0)
+    # keys of zero under the largest scales
+    c.k_scale.fill_(2.0 ** 119)
+    c.k.view(torch.uint8).zero_()
+    o, M = c.attend((q.double() * 2.0 ** 126).bfloat16(), table, ints(200), 0.125, return_stats=True)
+    check_decode(o, M, torch.zeros_like(q), c, table, lens, 0.125)

@@ -26,6 +26,8 @@
 // 24 sequences of 700 to 3900 tokens with 48/48 heads of 64 52 us = 5.0 TB/s, bound by its instructions (one query
 // row in eight uses what the softmax computes); 96 sequences of 40 to 8000 tokens at 32/4 heads 42 us = 3.8 TB/s (about
 // 750 chunks for 592 places); one of 1900 tokens 6.3 us, a row of latencies.
+#include <cfloat>
+
 #include "common.cuh"
 #include "serving.h"
 
@@ -403,10 +405,16 @@ __global__ void __launch_bounds__(THREADS, CTAS<D, NT>) attn_decode_kernel(const
 #pragma unroll
       for (int u = 0; u < SL; ++u) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int t = 0; t < NT; ++t) {
+          // the factors first: a large q over small keys (2^120 and 2^-120, say) is an ordinary score, its product with
+          // q's factor alone is infinite.  Finite, so that a product of 0 stays 0 under factors that pass fp32's range.
+          float f0, f1;
+          upk2(mul2(pk2(fac[t][0], fac[t][1]), pk2(ks[u], ks[u])), f0, f1);
+          const uint64_t f = pk2(fminf(f0, FLT_MAX), fminf(f1, FLT_MAX));
 #pragma unroll
           for (int j = 0; j < 4; j += 2)  // two query rows at a time
-            upk2(mul2(mul2(pk2(s[u][t][j], s[u][t][j + 1]), pk2(fac[t][0], fac[t][1])), pk2(ks[u], ks[u])), s[u][t][j], s[u][t][j + 1]);
+            upk2(mul2(pk2(s[u][t][j], s[u][t][j + 1]), f), s[u][t][j], s[u][t][j + 1]);
+        }
         if (left[u] < SLAB) {
 #pragma unroll
           for (int t = 0; t < NT; ++t)
