@@ -284,7 +284,8 @@ B200_API long long b200_attention_bwd_noalloc_capacity(void);
  * addresses 16-byte aligned; D is 64, 128 or 256.  m (may be NULL): [Hq, T] fp32, the base-2 log-sum-exp of
  * b200_attention_fwd.  Rows of o and m that belong to no sequence are left as they were (zero_rest = 0), set to
  * zero and -inf (zero_rest = 1), or left in o and set to -inf in m (zero_rest = 2).  Values of one sequence never reach another, infinities and NaN
- * included.  A launch draws a work counter like b200_attention_fwd's. */
+ * included.  A launch draws a work counter like b200_attention_fwd's; a captured one for which there is none left
+ * divides its work beforehand instead. */
 B200_API int b200_attention_varlen_fwd(b200_stream_t stream, const void* q, const void* k, const void* v, void* o,
                                        float* m, const int* cu_seqlens, int batch, int T, int Hq, int Hkv, int D,
                                        const int64_t stride_q[3], const int64_t stride_k[3], const int64_t stride_v[3],

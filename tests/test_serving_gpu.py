@@ -931,3 +931,61 @@ def test_decode_large_queries_over_small_keys():
     c.k.view(torch.uint8).zero_()
     o, M = c.attend((q.double() * 2.0 ** 126).bfloat16(), table, ints(200), 0.125, return_stats=True)
     check_decode(o, M, torch.zeros_like(q), c, table, lens, 0.125)
+
+
+CAPTURE_MANY = """
+import gc, time, torch, triton_b200 as tb
+dev = "cuda"
+g = torch.Generator(device=dev).manual_seed(1)
+q, k, v = (torch.randn(2000, h, 64, generator=g, device=dev).half() for h in (8, 2, 2))
+cu = torch.tensor([0, 1500, 1500, 2000], dtype=torch.int32, device=dev)
+want = tb.attention_varlen(q, k, v, cu, True, 0.1)
+dq, dk, dv = (torch.randn(1, 2, 300, 64, generator=g, device=dev).half() for _ in range(3))
+dwant = tb.attention_forward(dq, dk, dv, True, 0.1)[0]
+
+def capture(n, call, want):
+    outs, graph = [], torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for i in range(n):
+            o = call()
+            if i % 500 == 0:
+                outs.append(o)
+    for _ in range(2):
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+    return graph, outs
+
+packed = lambda: tb.attention_varlen(q, k, v, cu, True, 0.1)
+# graphs that are destroyed give their launches' counters back, packed and dense ones
+for call, w in ((packed, want), (lambda: tb.attention_forward(dq, dk, dv, True, 0.1)[0], dwant)):
+    for _ in range(3):
+        kept = capture(2000, call, w)
+        del kept
+        gc.collect()
+        torch.cuda.synchronize()
+        time.sleep(0.2)
+# more at a time than there are counters
+kept = [capture(1500, packed, want) for _ in range(3)]
+cu.copy_(torch.tensor([0, 0, 3, 2000], dtype=torch.int32))
+want = packed()
+for graph, outs in kept:
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+assert tb._lib.status() == 0
+print("fine")
+"""
+
+
+def test_captures_do_not_run_out_of_work_counters():
+    """More captured launches than the pool of work counters holds, one graph after another and at a time; in a
+    process of their own."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", CAPTURE_MANY], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("fine"), r.stdout + r.stderr

@@ -83,8 +83,9 @@ int launch_attn_varlen(DeviceCtx* ctx, cudaStream_t stream, const AttnVarlenArgs
   p.by_level = a.causal && (a.Hq > a.Hkv || (long long)a.T * a.Hkv * a.D * 4 <= (128 << 20) || (long long)a.T <= 1024LL * a.batch);
   p.rest = a.rest;
   p.status = ctx->status;
-  p.sched_counter = next_sched_counter(ctx, stream);
-  if (!p.sched_counter) return B200_ERR_CUDA;
+  bool used_up = false;
+  p.sched_counter = next_sched_counter(ctx, stream, &used_up);
+  if (!p.sched_counter && !used_up) return B200_ERR_CUDA;
   const long long most_items = ((long long)a.T / p.item_pos + a.batch) * p.block_items;  // the lengths are on the device
   const bool bf16 = a.dtype == B200_BF16;
   if (a.D == 256) return bf16 ? launch_packed_t<256, true>(ctx, stream, tq, tk, tv, to, p, most_items) : launch_packed_t<256, false>(ctx, stream, tq, tk, tv, to, p, most_items);

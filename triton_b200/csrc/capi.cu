@@ -24,8 +24,8 @@ __device__ __align__(16) unsigned g_status_word[4];
 // Eager launches take the next word of a ring, so launches in flight on different streams do not
 // share one (more than kSchedRing attention launches in flight at once on one device would).
 // Launches captured into a CUDA graph keep their counter for as long as the graph may be
-// replayed, so they take words of a pool that is never recycled: a replay can then never meet
-// an eager launch, or another graph, on its counter.
+// replayed, so they take words of a pool that come back when the graph is destroyed: a replay can then
+// never meet an eager launch, or another graph, on its counter.
 constexpr unsigned kSchedRing = 256, kSchedGraphPool = 4096;
 __device__ int g_sched_ring[kSchedRing + kSchedGraphPool];
 
@@ -142,34 +142,70 @@ DeviceCtx* ready_ctx() {
   return ctx;
 }
 
-int* next_sched_counter(DeviceCtx* ctx, cudaStream_t stream) {
+// The counters of captured launches that can be handed out: `fresh` have never been, `back` are those whose graph is
+// gone.  A lock of its own: the graph's destruction may call give_back from any thread, inside any CUDA call.
+struct GraphPool {
+  unsigned fresh, n_back;
+  unsigned short back[kSchedGraphPool];
+};
+static GraphPool g_graph_pool[64];
+static std::mutex g_graph_pool_mu;
+static void CUDART_CB give_back(void* which) {
+  const uintptr_t w = reinterpret_cast<uintptr_t>(which);
+  std::lock_guard<std::mutex> lk(g_graph_pool_mu);
+  GraphPool& pool = g_graph_pool[w / kSchedGraphPool];
+  pool.back[pool.n_back++] = (unsigned short)(w % kSchedGraphPool);
+}
+
+int* next_sched_counter(DeviceCtx* ctx, cudaStream_t stream, bool* used_up) {
   static int* base[64] = {};
-  static unsigned next_eager[64] = {}, next_graph[64] = {};
+  static unsigned next_eager[64] = {};
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  cudaGraph_t graph = nullptr;
   cudaError_t e = cudaStreamIsCapturing(stream, &cap);
+  if (e == cudaSuccess && cap == cudaStreamCaptureStatusActive) e = cudaStreamGetCaptureInfo(stream, &cap, nullptr, &graph);
   if (e != cudaSuccess) {
-    fail(B200_ERR_CUDA, "cudaStreamIsCapturing: %s", cudaGetErrorString(e));
+    fail(B200_ERR_CUDA, "stream capture: %s", cudaGetErrorString(e));
     return nullptr;
   }
-  std::lock_guard<std::mutex> lk(g_mu);
-  if (!base[ctx->device]) {
-    void* ptr = nullptr;
-    e = cudaGetSymbolAddress(&ptr, g_sched_ring);
-    if (e != cudaSuccess) {
-      fail(B200_ERR_CUDA, "cudaGetSymbolAddress(scheduler ring): %s", cudaGetErrorString(e));
-      return nullptr;
+  {
+    std::lock_guard<std::mutex> lk(g_mu);
+    if (!base[ctx->device]) {
+      void* ptr = nullptr;
+      e = cudaGetSymbolAddress(&ptr, g_sched_ring);
+      if (e != cudaSuccess) {
+        fail(B200_ERR_CUDA, "cudaGetSymbolAddress(scheduler ring): %s", cudaGetErrorString(e));
+        return nullptr;
+      }
+      base[ctx->device] = static_cast<int*>(ptr);
     }
-    base[ctx->device] = static_cast<int*>(ptr);
+    if (cap == cudaStreamCaptureStatusNone) return base[ctx->device] + (next_eager[ctx->device]++ % kSchedRing);
   }
-  if (cap == cudaStreamCaptureStatusNone) return base[ctx->device] + (next_eager[ctx->device]++ % kSchedRing);
-  if (next_graph[ctx->device] >= kSchedGraphPool) {
-    fail(B200_ERR_UNSUPPORTED,
-         "this process has captured %u attention launches into CUDA graphs on device %d; each keeps its work "
-         "counter for the life of the process and the pool holds no more",
-         kSchedGraphPool, ctx->device);
+  unsigned at;
+  {
+    std::lock_guard<std::mutex> lk(g_graph_pool_mu);
+    GraphPool& pool = g_graph_pool[ctx->device];
+    if (pool.n_back > 0) at = pool.back[--pool.n_back];
+    else if (pool.fresh < kSchedGraphPool) at = pool.fresh++;
+    else at = kSchedGraphPool;
+  }
+  if (at == kSchedGraphPool) {
+    if (used_up) *used_up = true;
+    else
+      fail(B200_ERR_UNSUPPORTED,
+           "CUDA graphs of this process hold %u captured attention launches on device %d; each keeps its work "
+           "counter until its graph is destroyed and the pool holds no more",
+           kSchedGraphPool, ctx->device);
     return nullptr;
   }
-  return base[ctx->device] + kSchedRing + next_graph[ctx->device]++;
+  // The graph (and what is instantiated from it, and its replays in flight) keeps the counter; should it not take
+  // it, the counter is this launch's for the life of the process.
+  void* which = reinterpret_cast<void*>((uintptr_t)ctx->device * kSchedGraphPool + at);
+  cudaUserObject_t object = nullptr;
+  if (graph && (cudaUserObjectCreate(&object, which, give_back, 1, cudaUserObjectNoDestructorSync) != cudaSuccess ||
+                cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove) != cudaSuccess))
+    cudaGetLastError();  // (a reference that the graph has not taken stays: releasing it would give the counter back)
+  return base[ctx->device] + kSchedRing + at;
 }
 
 bool encode_tmap(CUtensorMap* out, int dtype, int rank, const void* base, const uint64_t* dims,

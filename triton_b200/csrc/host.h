@@ -30,9 +30,10 @@ DeviceCtx* current_ctx();
 DeviceCtx* ready_ctx();
 
 // A work counter (zero between launches: the kernel restores it) for one launch of a persistent kernel on
-// `stream`; launches under stream capture get counters that are never handed out again (nullptr + error
-// string on failure).
-int* next_sched_counter(DeviceCtx* ctx, cudaStream_t stream);
+// `stream`; launches under stream capture get counters of their own until their graph is destroyed
+// (nullptr + error string on failure).  `used_up` (may be nullptr): set where the capture pool holds no more, which is then no
+// failure: for a kernel that can do without.
+int* next_sched_counter(DeviceCtx* ctx, cudaStream_t stream, bool* used_up = nullptr);
 
 // Record an error message for b200_last_error() and return `code`.
 int fail(int code, const char* fmt, ...);
