@@ -989,3 +989,27 @@ def test_captures_do_not_run_out_of_work_counters():
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", CAPTURE_MANY], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip().endswith("fine"), r.stdout + r.stderr
+
+
+def test_calls_count_as_changes_of_what_they_write():
+    """autograd's version counters: a tensor saved for a backward and then written by a call is noticed."""
+    q, k, v, cu, off = pack([20, 60], 4, 2, 64, torch.float16, seed=171)
+    c = tb.PagedKVCache(8, 16, 2, 64)
+    table, lens = torch.arange(8, dtype=I32, device=DEV).view(2, 4), ints(20, 60)
+    w = torch.ones_like(c.k_scale, requires_grad=True)
+    y = (w * c.k_scale).sum()
+    c.append(k, v, table, lens, cu)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    for t in (c.k, c.v, c.k_scale, c.v_scale):
+        assert t._version > 0
+    mine = torch.zeros_like(q)
+    tb.attention_varlen(q, k, v, cu, True, 0.1, out=mine)
+    one = torch.zeros(2, 4, 64, device=DEV).half()
+    c.attend(q[:2], table, lens, 0.1, out=one)
+    assert mine._version == 1 and one._version == 1
+    with torch.inference_mode():
+        d = tb.PagedKVCache(8, 16, 2, 64)
+        d.append(k, v, table, lens, cu)
+        tb.attention_varlen(q, k, v, cu, True, 0.1, out=torch.zeros_like(q))
+        assert torch.equal(d.k.view(torch.uint8), c.k.view(torch.uint8))

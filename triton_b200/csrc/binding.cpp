@@ -65,6 +65,11 @@ c10::Device one_device(std::initializer_list<const Tensor*> ts) {
 b200_stream_t stream_of(c10::Device dev) {
   return reinterpret_cast<b200_stream_t>(c10::cuda::getCurrentCUDAStream(dev.index()).stream());
 }
+// what a call has written counts as changed for autograd's saved tensors (inference tensors keep no count)
+void changed(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
 bool half_type(const Tensor& t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
 int dtype_of(const Tensor& t) { return t.scalar_type() == at::kHalf ? B200_F16 : B200_BF16; }
 int small(int64_t n) {
@@ -106,6 +111,7 @@ py::object attention_varlen(const Tensor& q, const Tensor& k, const Tensor& v, c
                    small(Hq), small(Hkv), small(D), q.strides().data(), k.strides().data(), v.strides().data(),
                    o.strides().data(), static_cast<float>(sm_scale), causal, dtype_of(q), out ? 2 : 1),
         "attention_varlen");
+  if (out) changed({&*out});
   return result(o, m, stats);
 }
 
@@ -149,6 +155,7 @@ void kv_cache_append(const Tensor& k_cache, const Tensor& v_cache, const Tensor&
                   cu ? cu->const_data_ptr<int>() : nullptr, small(batch), small(k.size(0)), c.heads, c.D, k.strides().data(),
                   v.strides().data(), dtype_of(k)),
         "kv_cache_append");
+  changed({&k_cache, &v_cache, &k_scale, &v_scale});
 }
 
 py::object attention_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale,
@@ -175,6 +182,7 @@ py::object attention_decode(const Tensor& q, const Tensor& k_cache, const Tensor
                stats ? m.mutable_data_ptr<float>() : nullptr, batch, Hq, c.heads, c.D, q.strides().data(), o.strides().data(),
                static_cast<float>(sm_scale), dtype_of(q), bytes ? ws.mutable_data_ptr() : nullptr),
         "attention_decode");
+  if (out) changed({&*out});
   return result(o, m, stats);
 }
 
