@@ -1013,3 +1013,47 @@ def test_calls_count_as_changes_of_what_they_write():
         d.append(k, v, table, lens, cu)
         tb.attention_varlen(q, k, v, cu, True, 0.1, out=torch.zeros_like(q))
         assert torch.equal(d.k.view(torch.uint8), c.k.view(torch.uint8))
+
+
+def test_calls_refuse_outputs_that_overlap():
+    """An `out` whose elements share memory, or that lies over k, v or the cache, would be written while it is read."""
+    q, k, v, cu, off = pack([20, 60], 2, 2, 64, torch.float16, seed=181)
+    want = tb.attention_varlen(q, k, v, cu, True, 0.1)
+    kept = k.clone(), v.clone()
+    for out in (k, v, torch.zeros(1, 2, 64, device=DEV).half().expand(80, 2, 64), torch.zeros(80, 1, 64, device=DEV).half().expand(80, 2, 64)):
+        with pytest.raises(RuntimeError):
+            tb.attention_varlen(q, k, v, cu, True, 0.1, out=out)
+    assert torch.equal(k, kept[0]) and torch.equal(v, kept[1])
+    c, table = filled_cache([20, 60], 2, 16, 64, seed=182)
+    x = q[:2].clone()
+    one = c.attend(x, table, ints(20, 60), 0.1)
+    with pytest.raises(RuntimeError):
+        c.attend(x, table, ints(20, 60), 0.1, out=torch.zeros(1, 2, 64, device=DEV).half().expand(2, 2, 64))
+    # q itself may take the output: a row of it is read by the tile that writes it
+    assert torch.equal(c.attend(x, table, ints(20, 60), 0.1, out=x), one)
+    assert torch.equal(tb.attention_varlen(q, k, v, cu, True, 0.1, out=q), want)
+
+
+def test_inputs_whose_elements_share_memory():
+    """Heads or rows expanded from one: a stride of zero."""
+    q, k, v, cu, off = pack([20, 60], 4, 1, 128, torch.bfloat16, seed=191)
+    wide = lambda t: t.expand(80, 2, 128)
+    want = tb.attention_varlen(q, wide(k).contiguous(), wide(v).contiguous(), cu, True, 0.1)
+    assert torch.equal(tb.attention_varlen(q, wide(k), wide(v), cu, True, 0.1), want)
+    one_q = q[:1].expand(80, 4, 128)
+    assert torch.equal(tb.attention_varlen(one_q, k, v, cu, True, 0.1), tb.attention_varlen(one_q.contiguous(), k, v, cu, True, 0.1))
+    a, b = tb.PagedKVCache(8, 16, 2, 128), tb.PagedKVCache(8, 16, 2, 128)
+    table, lens = torch.arange(8, dtype=I32, device=DEV).view(2, 4), ints(20, 60)
+    a.append(wide(k), wide(v), table, lens, cu)
+    b.append(wide(k).contiguous(), wide(v).contiguous(), table, lens, cu)
+    assert torch.equal(a.k.view(torch.uint8), b.k.view(torch.uint8)) and torch.equal(a.v_scale, b.v_scale)
+    x = q[:1].expand(2, 4, 128)
+    assert torch.equal(a.attend(x, table, lens, 0.1), a.attend(x.contiguous(), table, lens, 0.1))
+
+
+def test_out_of_memory_is_torchs():
+    """An output that cannot be had is torch's OutOfMemoryError, as everywhere else."""
+    q = torch.zeros(1, 1, 64, device=DEV).half().expand(1 << 20, 1 << 16, 64)
+    k = torch.zeros(1, 1, 64, device=DEV).half().expand(1 << 20, 1, 64)
+    with pytest.raises(torch.OutOfMemoryError):
+        tb.attention_varlen(q, k, k, ints(0, 1), True, 0.1)

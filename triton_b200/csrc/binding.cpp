@@ -5,6 +5,7 @@
 //
 // The C ABI's functions come as addresses from the Python side (bind), so that whichever build of the
 // library _lib.py has loaded is the one that runs.
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -84,6 +85,9 @@ Tensor output(const optional<Tensor>& out, const Tensor& q, c10::Device dev) {
   if (!out) return at::empty(q.sizes(), at::TensorOptions().dtype(q.scalar_type()).device(dev));
   require(out->sizes() == q.sizes() && out->scalar_type() == q.scalar_type() && out->device() == dev, "out= must look like q");
   no_grad("out=", {&*out});
+  // q itself may take the output: what writes a row has read it.  Anything else that shares memory is read by others.
+  at::assert_no_internal_overlap(*out);
+  at::assert_no_partial_overlap(*out, q);
   return *out;
 }
 py::object result(const Tensor& o, const Tensor& m, bool stats) {
@@ -104,6 +108,10 @@ py::object attention_varlen(const Tensor& q, const Tensor& k, const Tensor& v, c
   const c10::Device dev = one_device({&q, &k, &v, &cu});
   c10::cuda::CUDAGuard guard(dev);
   const Tensor o = output(out, q, dev);
+  if (out) {
+    at::assert_no_overlap(o, k);
+    at::assert_no_overlap(o, v);
+  }
   Tensor m;
   if (stats) m = at::empty({Hq, T}, at::TensorOptions().dtype(at::kFloat).device(dev));
   check(varlen_fwd(stream_of(dev), q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), o.mutable_data_ptr(),

@@ -30,7 +30,7 @@ def attention_varlen(q, k, v, cu_seqlens, causal, sm_scale, *, out=None, return_
     others multiples of 8 (slices of one fused projection, say).  Returns O [T, Hq, D], with
     return_stats=True (O, M): M [Hq, T] is the base-2 log-sum-exp of attention_forward.
     Rows of T that belong to no sequence (padding behind the last one) come back as zeros, with `out=` they stay
-    as they were; in M they are -inf.
+    as they were; in M they are -inf.  `out` may be q, but not share memory with k or v.
     """
     if q.dim() == 3 and q.shape[2] in (16, 32):  # as in attention_forward: zero-padded to the kernels' head dim 64
         D = q.shape[2]
