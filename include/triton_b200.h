@@ -279,7 +279,7 @@ B200_API long long b200_attention_bwd_noalloc_capacity(void);
 /* Attention of whole prompts packed behind one another, with grouped heads: q, o [T, Hq, D] and k, v
  * [T, Hkv, D] of `dtype` (F16 or BF16), Hq a multiple of Hkv, query head h reads k/v head h / (Hq / Hkv);
  * sequence b is the rows cu_seqlens[b] .. cu_seqlens[b + 1] (a DEVICE array of batch + 1 ints that do not
- * decrease; what lies outside [0, T] is cut off).  Each sequence attends to itself, up to the row itself
+ * decrease; what lies outside [0, T] is cut off; of overlapping sequences with 2^31 work items nothing is computed).  Each sequence attends to itself, up to the row itself
  * when `causal`.  Strides are {token, head, d} in elements, the d stride 1, the others multiples of 8; base
  * addresses 16-byte aligned; D is 64, 128 or 256.  m (may be NULL): [Hq, T] fp32, the base-2 log-sum-exp of
  * b200_attention_fwd.  Rows of o and m that belong to no sequence are left as they were (zero_rest = 0), set to

@@ -1057,3 +1057,20 @@ def test_out_of_memory_is_torchs():
     k = torch.zeros(1, 1, 64, device=DEV).half().expand(1 << 20, 1, 64)
     with pytest.raises(torch.OutOfMemoryError):
         tb.attention_varlen(q, k, k, ints(0, 1), True, 0.1)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_varlen_offsets_that_name_the_same_rows_over_and_over(causal):
+    """Decreasing offsets that add up to more work than an int counts: no work, and nothing breaks."""
+    T, H, batch = 16384, 32, (1 << 21) + 2
+    q = torch.zeros(T, H, 64, dtype=torch.float16, device=DEV)
+    cu = torch.zeros(batch + 1, dtype=I32, device=DEV)
+    cu[1::2] = T
+    mine = torch.full_like(q, 7.0)
+    tb.attention_varlen(q, q, q, cu, causal, 0.1, out=mine)
+    torch.cuda.synchronize()
+    assert _lib.status() == 0 and (mine == 7.0).all()
+    # a few of them are fine: the same rows, computed twice
+    q.normal_(generator=torch.Generator(device=DEV).manual_seed(1))
+    o = tb.attention_varlen(q[:300], q[:300], q[:300], ints(0, 300, 0, 300), causal, 0.1)
+    assert torch.equal(o, tb.attention_varlen(q[:300], q[:300], q[:300], ints(0, 300), causal, 0.1))

@@ -95,6 +95,7 @@ struct PackedFwdParams : FwdParams {
   int tile_pos;      // positions of a tile: 128 / fold
   int item_pos, item_shift;    // positions of an item, and their log2 (-1: no power of two)
   int block_items, kv_items;   // items per block of item_pos positions, and of those per k/v head
+  int lane_most;     // (2^26 - 1) / block_items, see PackedWalk::init
   int rest;          // rows that belong to no sequence: bit 0 set to zero in o, bit 1 set to -inf in m
 };
 
@@ -202,9 +203,13 @@ struct PackedWalk {
     start0 = len0 = 0;
     if ((int)(threadIdx.x & 31) < p.batch) extent(p, threadIdx.x & 31, start0, len0);
     blocks0 = blocks_of(p, len0);
+    // Decreasing offsets can name the same rows over and over, up to more tickets than an int counts: of such a pack
+    // nothing is computed.  (32 lanes of lane_most are still below 2^31; a pack that takes its rows once has fewer in
+    // one lane, or its o were a terabyte.)
     int sum = 0;
-    for (int b = threadIdx.x & 31; b < p.batch; b += 32) sum += seq_blocks(p, b);
+    for (int b = threadIdx.x & 31; b < p.batch; b += 32) sum = min(sum + seq_blocks(p, b), 1 << 30);
     total = (int)__reduce_add_sync(0xffffffffu, (unsigned)sum) * p.block_items;
+    if (__any_sync(0xffffffffu, sum > p.lane_most)) total = 0;
     base = 0;
     enter(p, 0x7fffffff);
   }

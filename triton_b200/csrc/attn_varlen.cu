@@ -81,6 +81,7 @@ int launch_attn_varlen(DeviceCtx* ctx, cudaStream_t stream, const AttnVarlenArgs
   // 528 us), unless the sequences have few levels (64 x 512 at 32/32: 273 against 295).  Not causal, every block
   // of a sequence costs the same and only the reuse counts (4 x 4096 at 32/32: 1063 against 882 us).
   p.by_level = a.causal && (a.Hq > a.Hkv || (long long)a.T * a.Hkv * a.D * 4 <= (128 << 20) || (long long)a.T <= 1024LL * a.batch);
+  p.lane_most = ((1 << 26) - 1) / p.block_items;
   p.rest = a.rest;
   p.status = ctx->status;
   bool used_up = false;
