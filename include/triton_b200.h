@@ -285,7 +285,10 @@ B200_API long long b200_attention_bwd_noalloc_capacity(void);
  * b200_attention_fwd.  Rows of o and m that belong to no sequence are left as they were (zero_rest = 0), set to
  * zero and -inf (zero_rest = 1), or left in o and set to -inf in m (zero_rest = 2).  Values of one sequence never reach another, infinities and NaN
  * included.  A launch draws a work counter like b200_attention_fwd's; a captured one for which there is none left
- * divides its work beforehand instead. */
+ * divides its work beforehand instead.
+ * Scores, maxima and sums are fp32; the weights are rounded to `dtype` before they meet V (at head dims 128 and 256 a
+ * quarter of them come from a cubic for 2^x, within 8.6e-5) and summed before that rounding; o is rounded once.  Within
+ * a sequence a V that is not finite may reach rows before its own, too (0 * inf). */
 B200_API int b200_attention_varlen_fwd(b200_stream_t stream, const void* q, const void* k, const void* v, void* o,
                                        float* m, const int* cu_seqlens, int batch, int T, int Hq, int Hkv, int D,
                                        const int64_t stride_q[3], const int64_t stride_k[3], const int64_t stride_v[3],
@@ -315,8 +318,12 @@ B200_API int b200_kv_append(b200_stream_t stream, void* k_cache, void* v_cache, 
  * {sequence, head, d}, multiples of 8 but for d), over the first seq_lens[b] tokens of sequence b (cut at
  * max_pages * page_size).  m (may be NULL): [batch, Hq] fp32, base-2 log-sum-exp.  A sequence without tokens
  * gives zeros and -inf.  The launch covers max_pages * page_size tokens of every sequence (the lengths are
- * not known on the host): pass no more columns of the table than the longest sequence needs.  `workspace`: b200_attention_decode_workspace(...) bytes (0: none needed), 16-byte
- * aligned, the caller's scratch for the call; calls that may overlap need one each.  Bitwise repeatable. */
+ * not known on the host): pass no more columns of the table than the longest sequence needs.  `workspace`:
+ * b200_attention_decode_workspace(...) bytes (0: none needed), 16-byte aligned, the caller's scratch for the call; calls
+ * that may overlap need one each.  Bitwise repeatable.
+ * Only the exponents of the scales are read.  Scores, maxima and sums are fp32; the weights are rounded to fp16 before
+ * they meet V and summed before that rounding; a bf16 row of q is taken as fp16 times a power of two (what lies 2^-29
+ * below the row's largest value loses bits). */
 B200_API size_t b200_attention_decode_workspace(int batch, int Hq, int Hkv, int D, int page_size, int max_pages);
 B200_API int b200_attention_decode(b200_stream_t stream, const void* q, const void* k_cache, const void* v_cache,
                                    const float* k_scale, const float* v_scale, int pages, int page_size,

@@ -14,8 +14,10 @@
 //
 // Roundings to 16 bits: q in fp16 as it is, in bf16 times a power of two of its row that brings the row's
 // largest value near fp16's top (8 significant bits fit; what lies 2^-29 below the largest loses bits);
-// P to fp16, relative to a running reference that leaves weights 2^-7 .. 2^15 at the top, so that the
-// weights of a long flat cache stay normal beside one large key.  Scores, maxima, sums and O: fp32.
+// P to fp16, relative to a running reference that leaves the largest weight at 2^7 when it moves and lets it grow
+// to 2^15 before it moves again, so that the weights of a long flat cache stay normal beside one large key (down to
+// 2^-14, 21 log2 units below the largest just after a move).  The denominator sums the weights before this rounding.
+// Scores, maxima, sums and O: fp32.
 // The scale of V's page joins the weight's exponent before it is rounded (w = 2^(s + log2 vs - ref)), and
 // the denominator keeps a reference of its own, so pages of very different scales cannot overflow fp16.
 //

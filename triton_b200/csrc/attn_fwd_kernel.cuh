@@ -13,7 +13,7 @@
 //   warps 0-3 / 4-7   softmax of tile 0 / 1, one thread per query row (no cross-thread reduction):
 //                     tcgen05.ld S, running max and sum, exp2, P packed to 16 bit and written back over S in TMEM
 //                     (tcgen05.st) as the A operand of the second MMA.  The accumulator O is
-//                     rescaled lazily: only when the running max grew by more than 2^8 does the
+//                     rescaled lazily: only when the running max grew by more than kRescaleThreshold does the
 //                     warp multiply its O rows in TMEM (the reference rescales every step; the
 //                     result is the same up to fp32 rounding since P and l carry the same factor).
 //                     At the end: O / l -> storage type -> global, M -> global.

@@ -1,11 +1,12 @@
 """PyTorch custom-op registration of the library's entry points.
 
 `torch.ops.triton_b200.matmul`, `.attention_fwd`, `.attention_bwd`, the differentiable `.attention` and the
-serving calls `.attention_varlen`, `.kv_cache_append` (in place) and `.attention_decode` are registered with `torch.library.custom_op`: they show up in the dispatcher, have
-fake (meta) implementations so that `torch.compile` / export can trace through them without
-running a kernel, and `attention` carries its backward formula.  The CUDA implementations are the
-functions of `triton_b200.ops` and `triton_b200.serving`, i.e. the C ABI of include/triton_b200.h through ctypes; there is
-no CPU implementation: on CPU tensors the ops raise, like the functions they wrap.
+serving calls `.attention_varlen`, `.kv_cache_append` (in place) and `.attention_decode` are registered with
+`torch.library.custom_op`: they show up in the dispatcher, have fake (meta) implementations so that
+`torch.compile` / export can trace through them without running a kernel, and `attention` carries its
+backward formula.  The CUDA implementations are the functions of `triton_b200.ops` (the C ABI of
+include/triton_b200.h through ctypes) and `triton_b200.serving` (the same through csrc/binding.cpp); there
+is no CPU implementation: on CPU tensors the ops raise, like the functions they wrap.
 """
 from typing import Optional, Tuple
 

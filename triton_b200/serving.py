@@ -31,6 +31,11 @@ def attention_varlen(q, k, v, cu_seqlens, causal, sm_scale, *, out=None, return_
     return_stats=True (O, M): M [Hq, T] is the base-2 log-sum-exp of attention_forward.
     Rows of T that belong to no sequence (padding behind the last one) come back as zeros, with `out=` they stay
     as they were; in M they are -inf.  `out` may be q, but not share memory with k or v.
+
+    Scores, their maximum and all sums are fp32.  The weights are rounded to the inputs' type before they meet V
+    (at head dims 128 and 256 a quarter of them come from a cubic for 2^x, within 8.6e-5), the output once more.
+    Sequences keep to themselves whatever their values; within one, a V that is not finite may also reach rows
+    before its own, whose weight for it is 0 (0 * inf).
     """
     if q.dim() == 3 and q.shape[2] in (16, 32):  # as in attention_forward: zero-padded to the kernels' head dim 64
         D = q.shape[2]
@@ -62,6 +67,9 @@ def attention_decode(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens
     of the cache's heads, over the first seq_lens[b] tokens (the new one among them, once it is appended).  Tokens
     of a page that the table does not name are left out; a sequence without tokens gives zeros.  Returns O like
     q, with return_stats=True (O, M): M [batch, Hq] is the base-2 log-sum-exp (-inf without tokens).
+    The scales have to be powers of two, as kv_cache_append leaves them: only their exponents are read.  Scores,
+    their maximum and all sums are fp32; the weights are rounded to fp16 before they meet V, and a bf16 row of q is
+    taken as fp16 times a power of two (what lies 2^-29 below the row's largest value loses bits).
     The lengths stay on the GPU, so the launch covers what the table has room for: where that is far more than
     the longest sequence, pass its first columns (page_table[:, :n])."""
     return (_lib._binding or _lib.binding()).attention_decode(q, k_cache, v_cache, k_scale, v_scale, page_table, seq_lens, sm_scale,
